@@ -9,9 +9,11 @@ from __future__ import annotations
 
 import ctypes as C
 
-F32, F16, Q8_0 = 0, 1, 8
-TYPE_NAMES = {F32: "f32", F16: "f16", Q8_0: "q8_0"}
+F32, F16, Q4_0, Q8_0 = 0, 1, 2, 8
+TYPE_NAMES = {F32: "f32", F16: "f16", Q4_0: "q4_0", Q8_0: "q8_0"}
 QK8_0, Q8_0_BLOCK_BYTES = 32, 34
+BLOCK_BYTES = {Q4_0: 18, Q8_0: 34}   # of 32 values
+ROPE_NORM, ROPE_NEOX = 0, 2
 
 OK = 0
 E_NULL, E_TYPE, E_SHAPE, E_STRIDE, E_ALIGN, E_UNSUPPORTED = -1, -2, -3, -4, -5, -6
@@ -67,6 +69,17 @@ class KvConfig(C.Structure):
     ]
 
 
+class RopeParams(C.Structure):
+    _fields_ = [
+        ("n_dims", C.c_int32),
+        ("mode", C.c_int32),
+        ("freq_base", C.c_float),
+        ("freq_scale", C.c_float),
+        ("eps", C.c_float),
+        ("reserved", C.c_int32),
+    ]
+
+
 class TraceRecord(C.Structure):
     _fields_ = [("kernel", C.c_int32), ("n_splits", C.c_int32), ("head_dim", C.c_int32), ("q_len", C.c_int32),
                 ("kv_len", C.c_int32), ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("n_batch", C.c_int32),
@@ -111,6 +124,10 @@ SYMBOLS = {
     "b200_kv_bytes": (C.c_size_t, [C.c_void_p]),
     "b200_kv_view": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, TP, TP]),
     "b200_kv_append": (C.c_int, [C.c_void_p, C.c_int, TP, TP, C.c_void_p, C.c_int32, C.c_void_p]),
+    "b200_kv_read": (C.c_int, [C.c_void_p, C.c_int, TP, TP, C.c_void_p, C.c_int32, C.c_void_p]),
+    "b200_qk_norm_rope": (C.c_int, [TP, TP, TP, TP, C.POINTER(RopeParams), C.c_void_p, C.c_int32, C.c_void_p, TP, TP, C.c_void_p]),
+    "b200_kv_append_rope": (C.c_int, [C.c_void_p, C.c_int, TP, TP, TP, TP, TP, C.POINTER(RopeParams), C.c_void_p, C.c_int32, C.c_void_p, TP,
+                                      C.c_void_p]),
     "b200_kv_copy_stream": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int64, C.c_void_p]),
     "b200_beam_cells_to_index": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p]),
     "b200_mask_classify": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
@@ -149,14 +166,14 @@ def bind(lib: C.CDLL, symbols=SYMBOLS) -> C.CDLL:
 
 
 def _elem_size(t: int) -> int:
-    return {F32: 4, F16: 2, Q8_0: Q8_0_BLOCK_BYTES}[t]
+    return {F32: 4, F16: 2, **BLOCK_BYTES}[t]
 
 
 def describe(ptr: int, type_: int, shape, strides_bytes) -> Tensor:
     """Build a descriptor from a slowest-first shape/byte-stride pair (numpy/torch order).
 
-    For Q8_0 the caller passes the LOGICAL shape (elements) with strides of the block storage:
-    the fastest stride must be 34 (one block) and the fastest extent counts elements.
+    For Q8_0 and Q4_0 the caller passes the LOGICAL shape (elements) with strides of the block storage:
+    the fastest stride must be 34 or 18 (one block) and the fastest extent counts elements.
     """
     nd = len(shape)
     if nd > 4:
@@ -172,7 +189,7 @@ def describe(ptr: int, type_: int, shape, strides_bytes) -> Tensor:
     nb[0] = _elem_size(type_) if nd == 0 else nb[0]
     # ggml fills strides of absent (size-1) trailing dimensions with the full extent
     for i in range(max(nd, 1), 4):
-        prev_rows = ne[i - 1] if not (type_ == Q8_0 and i - 1 == 0) else ne[0] // QK8_0
+        prev_rows = ne[i - 1] if not (type_ in BLOCK_BYTES and i - 1 == 0) else ne[0] // QK8_0
         nb[i] = nb[i - 1] * prev_rows
     for i in range(4):
         t.ne[i] = ne[i]
@@ -181,34 +198,34 @@ def describe(ptr: int, type_: int, shape, strides_bytes) -> Tensor:
 
 
 def from_numpy(a, type_: int | None = None, logical_last: int | None = None) -> Tensor:
-    """Describe a numpy array. uint8 arrays with type_=Q8_0 hold blocks: the last axis is bytes
-    (a multiple of 34) and ``logical_last`` (default bytes/34*32) is the element count."""
+    """Describe a numpy array. uint8 arrays with type_=Q8_0 or Q4_0 hold blocks: the last axis is bytes
+    (a multiple of 34 or 18) and ``logical_last`` (default bytes/34*32, bytes/18*32) is the element count."""
     import numpy as np
 
     if type_ is None:
         type_ = {np.dtype(np.float32): F32, np.dtype(np.float16): F16}[a.dtype]
-    if type_ == Q8_0:
+    if type_ in BLOCK_BYTES:
         if a.dtype != np.uint8 or a.strides[-1] != 1:
-            raise ValueError("Q8_0 arrays are uint8 with a contiguous last axis")
-        n = logical_last if logical_last is not None else a.shape[-1] // Q8_0_BLOCK_BYTES * QK8_0
+            raise ValueError(f"{TYPE_NAMES[type_].upper()} arrays are uint8 with a contiguous last axis")
+        n = logical_last if logical_last is not None else a.shape[-1] // BLOCK_BYTES[type_] * QK8_0
         shape = list(a.shape[:-1]) + [n]
-        strides = list(a.strides[:-1]) + [Q8_0_BLOCK_BYTES]
-        return describe(a.ctypes.data, Q8_0, shape, strides)
+        strides = list(a.strides[:-1]) + [BLOCK_BYTES[type_]]
+        return describe(a.ctypes.data, type_, shape, strides)
     return describe(a.ctypes.data, type_, a.shape, a.strides)
 
 
 def from_torch(x, type_: int | None = None) -> Tensor:
-    """Describe a torch tensor (any device). uint8 tensors with type_=Q8_0 hold blocks."""
+    """Describe a torch tensor (any device). uint8 tensors with type_=Q8_0 or Q4_0 hold blocks."""
     import torch
 
     if type_ is None:
         type_ = {torch.float32: F32, torch.float16: F16}[x.dtype]
     es = x.element_size()
     strides = [s * es for s in x.stride()]
-    if type_ == Q8_0:
+    if type_ in BLOCK_BYTES:
         if x.dtype != torch.uint8 or x.stride(-1) != 1:
-            raise ValueError("Q8_0 tensors are uint8 with a contiguous last axis")
-        shape = list(x.shape[:-1]) + [x.shape[-1] // Q8_0_BLOCK_BYTES * QK8_0]
-        strides = strides[:-1] + [Q8_0_BLOCK_BYTES]
-        return describe(x.data_ptr(), Q8_0, shape, strides)
+            raise ValueError(f"{TYPE_NAMES[type_].upper()} tensors are uint8 with a contiguous last axis")
+        shape = list(x.shape[:-1]) + [x.shape[-1] // BLOCK_BYTES[type_] * QK8_0]
+        strides = strides[:-1] + [BLOCK_BYTES[type_]]
+        return describe(x.data_ptr(), type_, shape, strides)
     return describe(x.data_ptr(), type_, x.shape, strides)

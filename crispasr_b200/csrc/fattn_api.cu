@@ -67,6 +67,7 @@ size_t type_size(int t) {
         case B200_TYPE_F32: return 4;
         case B200_TYPE_F16: return 2;
         case B200_TYPE_Q8_0: return 34;
+        case B200_TYPE_Q4_0: return 18;
         default: return 0;
     }
 }
@@ -87,13 +88,13 @@ View make_view(const b200_tensor* t) {
 }
 
 // Type, nb[0], alignment and stride-granularity rules of one operand.
-int check_operand(const b200_tensor* t, bool allow_f32, bool allow_f16, bool allow_q8) {
+int check_operand(const b200_tensor* t, bool allow_f32, bool allow_f16, bool allow_blocks) {
     if (!t->data) return B200_E_NULL;
     const size_t es = type_size(t->type);
     if (es == 0) return B200_E_TYPE;
     if (t->type == B200_TYPE_F32 && !allow_f32) return B200_E_TYPE;
     if (t->type == B200_TYPE_F16 && !allow_f16) return B200_E_TYPE;
-    if (t->type == B200_TYPE_Q8_0 && !allow_q8) return B200_E_TYPE;
+    if (is_blocks(t->type) && !allow_blocks) return B200_E_TYPE;
     if (t->nb[0] != es) return B200_E_STRIDE;
     const size_t align = t->type == B200_TYPE_F32 ? 4 : 2;
     if ((uintptr_t)t->data % align) return B200_E_ALIGN;
@@ -101,7 +102,7 @@ int check_operand(const b200_tensor* t, bool allow_f32, bool allow_f16, bool all
         if (t->nb[i] % align) return B200_E_STRIDE;
     for (int i = 0; i < 4; i++)
         if (t->ne[i] <= 0) return B200_E_SHAPE;
-    if (t->type == B200_TYPE_Q8_0 && t->ne[0] % 32) return B200_E_SHAPE;
+    if (is_blocks(t->type) && t->ne[0] % 32) return B200_E_SHAPE;
     return B200_OK;
 }
 
@@ -279,7 +280,7 @@ int make_plan(const b200_tensor* q, const b200_tensor* k, const b200_tensor* v, 
     plan->cast_each = plan->cast_r_bytes = 0;
     if (kernel == B200_KERNEL_TILE_MMA && override_k != B200_KERNEL_TILE_MMA && !decode_ok && (a.hd == 64 || a.hd == 128) &&
         !tc5_ok) {
-        // F32 / Q8_0 / unaligned K/V: a conversion pre-pass into the workspace puts the call on the tcgen05 kernel
+        // F32 / Q8_0 / Q4_0 / unaligned K/V: a conversion pre-pass into the workspace puts the call on the tcgen05 kernel
         FattnArgs c = kv_is_tma_ready(a) ? a : with_f16_kv(a, (const void*)256, (const void*)256);
         if (!r_is_tma_ready(a)) c = with_f16_r(c, (const void*)256);
         if (tc5_supported(c)) {
@@ -476,7 +477,7 @@ void* mapped_host(void* p, size_t bytes) {
 // Bytes spanned by a strided tensor (offset of the last element + one element/block).
 size_t span_bytes(const b200_tensor* t) {
     size_t last = 0;
-    const int64_t n0 = t->type == B200_TYPE_Q8_0 ? t->ne[0] / 32 : t->ne[0];
+    const int64_t n0 = is_blocks(t->type) ? t->ne[0] / 32 : t->ne[0];
     last += (size_t)(n0 - 1) * t->nb[0];
     for (int i = 1; i < 4; i++) last += (size_t)(t->ne[i] - 1) * t->nb[i];
     return last + t->nb[0];

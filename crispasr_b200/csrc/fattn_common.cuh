@@ -9,6 +9,9 @@
 
 namespace b200 {
 
+// Types whose rows are blocks of 32 values.
+__host__ __device__ constexpr bool is_blocks(int type) { return type == B200_TYPE_Q8_0 || type == B200_TYPE_Q4_0; }
+
 // One operand as the kernels see it: base pointer plus byte strides of dims 1..3.
 struct View {
     const uint8_t* p;

@@ -1,7 +1,7 @@
 // fattn_mma.cu — the general tiled attention kernel and the split-KV decode kernel.
 //
 // Both kernels stage K/V tiles as fp16 in XOR-swizzled shared memory (F16 rows are copied,
-// F32 rows are rounded, Q8_0 blocks are dequantised as fp32(d)*q and rounded to fp16), run
+// F32 rows are rounded, Q8_0 and Q4_0 blocks are dequantised as fp32(d)*q and rounded to fp16), run
 // Q.K^T and P.V on the mma.sync m16n8k16 tensor path with fp32 accumulators and keep the
 // online softmax in fp32 registers.
 //
@@ -82,6 +82,22 @@ __device__ __forceinline__ uint4 load8_as_half(const uint8_t* rowp, int type, in
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 f[i] = (c0 + i < hd) ? *reinterpret_cast<const float*>(rowp + 4 * (c0 + i)) : 0.0f;
+        }
+        out.x = pack_half2(f[0], f[1]);
+        out.y = pack_half2(f[2], f[3]);
+        out.z = pack_half2(f[4], f[5]);
+        out.w = pack_half2(f[6], f[7]);
+    } else if (type == B200_TYPE_Q4_0) {  // 18-byte blocks {fp16 d; 16 bytes of nibbles}; rows are only 2-byte aligned
+        const uint8_t* blk = rowp + 18 * (c0 >> 5);
+        const float d = __half2float(*reinterpret_cast<const __half*>(blk));
+        const uint16_t* qs = reinterpret_cast<const uint16_t*>(blk + 2 + (c0 & 15));   // values 16.. of a block: the high nibbles
+        const int sh = (c0 & 16) ? 4 : 0;
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t w = (uint32_t)qs[i] >> sh;
+            f[2 * i] = d * (float)((int)(w & 15u) - 8);
+            f[2 * i + 1] = d * (float)((int)((w >> 8) & 15u) - 8);
         }
         out.x = pack_half2(f[0], f[1]);
         out.y = pack_half2(f[2], f[3]);
@@ -2134,6 +2150,7 @@ int launch_cast_any(const View& k, void* kdst, const View& v, void* vdst, int n,
                                                             : launch_cast<B200_TYPE_F32, false>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st));
         case B200_TYPE_Q8_0: return (int)(words(k) && words(v) ? launch_cast<B200_TYPE_Q8_0, true>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st)
                                                                : launch_cast<B200_TYPE_Q8_0, false>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st));
+        case B200_TYPE_Q4_0: return (int)launch_cast<B200_TYPE_Q4_0, false>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st);
         default: return (int)(k.vec16 && v.vec16 ? launch_cast<B200_TYPE_F16, true>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st)
                                                  : launch_cast<B200_TYPE_F16, false>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st));
     }

@@ -1,0 +1,164 @@
+// kv_rows.cuh — eight values of a row per lane into a row of a KV cache (F16, Q8_0, Q4_0), and out of one.
+#pragma once
+
+#include "fattn_common.cuh"
+
+namespace b200 {
+
+constexpr size_t kv_row_bytes(int type, int hd) {
+    return type == B200_TYPE_F16 ? (size_t)hd * 2 : (size_t)hd / 32 * (type == B200_TYPE_Q8_0 ? 34 : 18);
+}
+
+// (int)roundf(t) for |t| < 2^22 without either unit's conversions: |t| + 1/2 truncated to an integer by two additions that
+// round towards zero (the first cannot reach an integer the exact sum does not reach), then the sign; NaN gives 0.  In a block
+// of values below 4e-37 1/d is beyond a float and t infinite: the low byte is that of the saturated conversion, 0xFF for
+// +inf, 0 for -inf (a branch for such blocks cost 0.2 us per launch).
+__device__ __forceinline__ uint32_t round_away(float t) {
+    asm("min.NaN.f32 %0, %0, 0f437F0000;" : "+f"(t));   // 255; a NaN stays one
+    const float m = fmaxf(fabsf(t), 0.0f);
+    const int32_t k = __float_as_int(__fadd_rz(__fadd_rz(m, 0.5f), 8388608.0f)), sign = __float_as_int(t) >> 31;
+    return (uint32_t)((k ^ sign) - sign);
+}
+// Low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// trunc(x * id + 8.5) clamped to [0, 15], in the low four bits: the sum is rounded towards zero, which no integer lies in the
+// way of, so the result is that of the exact sum; a second such addition leaves the integer in the low bits.  NaN gives 0.
+__device__ __forceinline__ uint32_t nibble_of(float x, float id) {
+    const float t = fminf(fmaxf(__fmaf_rz(x, id, 8.5f), 0.0f), 15.5f);
+    return (uint32_t)__float_as_int(__fadd_rz(t, 8388608.0f));
+}
+
+// Eight values f of a row, [c, c + 8), into the cache row at row_out.  All lanes of the warp call it, four neighbouring lanes
+// (from a multiple of four) having the values of a block of 32; a lane that is not `live` stores nothing.
+//
+// Q8_0 blocks, bit-identical to gguf-py quantize_blocks: d = amax/127 (fp32), stored as fp16; q = roundf(x * (1/d)) with
+// 1/d = 0 for d == 0.  A block is 34 bytes.  In a row of an even number of blocks (head_dim 64 / 128: rows start on a 4-byte
+// boundary) the quants of the odd blocks fill aligned words and those of the even ones straddle them by two bytes; there a lane
+// takes the upper half of its left neighbour's last word (the first lane the scale) and the row leaves in 32-bit stores.
+//
+// Q4_0 blocks: d = m / -8 (fp32), stored as fp16, m the first of the values of largest magnitude; q = trunc(x * (1/d) + 8.5), at
+// most 15.  Byte i holds values i and 16 + i: the lanes with values 0..15 and 16..31 exchange half of their nibbles, after which
+// each of the four has a word of the block's 16 bytes.
+template <int TYPE>
+__device__ __forceinline__ void store_row8(uint8_t* row_out, int c, const float (&f)[8], bool live, int hd) {
+    if constexpr (TYPE == B200_TYPE_F16) {
+        if (live)
+            *reinterpret_cast<uint4*>(row_out + c * 2) =
+                make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
+    } else {
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(f[i]));
+        const float own = amax;
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int blk = c >> 5, i4 = (c & 31) >> 3;   // lane i4 of the block's four
+        if constexpr (TYPE == B200_TYPE_Q8_0) {
+            const float d = __fdiv_rn(amax, 127.0f);
+            const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+            uint32_t q[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) q[i] = round_away(__fmul_rn(f[i], id));
+            const uint32_t w0 = low_bytes(q[0], q[1], q[2], q[3]), w1 = low_bytes(q[4], q[5], q[6], q[7]);
+            const uint32_t dbits = __half_as_ushort(__float2half_rn(d));
+            const uint32_t left = __shfl_up_sync(0xffffffffu, w1, 1);
+            if (!live) return;
+            uint8_t* out = row_out + blk * 34 + 8 * i4;
+            if ((hd & 63) == 0) {
+                if (blk & 1) {
+                    *reinterpret_cast<uint32_t*>(out + 2) = w0;
+                    *reinterpret_cast<uint32_t*>(out + 6) = w1;
+                    if (i4 == 0) *reinterpret_cast<uint16_t*>(out) = (uint16_t)dbits;
+                } else {
+                    *reinterpret_cast<uint32_t*>(out) = (w0 << 16) | (i4 == 0 ? dbits : left >> 16);
+                    *reinterpret_cast<uint32_t*>(out + 4) = __funnelshift_l(w0, w1, 16);
+                    if (i4 == 3) *reinterpret_cast<uint16_t*>(out + 8) = (uint16_t)(w1 >> 16);
+                }
+            } else {   // an odd number of blocks: rows are only 2-byte aligned
+                *reinterpret_cast<uint16_t*>(out + 2) = (uint16_t)w0;
+                *reinterpret_cast<uint16_t*>(out + 4) = (uint16_t)(w0 >> 16);
+                *reinterpret_cast<uint16_t*>(out + 6) = (uint16_t)w1;
+                *reinterpret_cast<uint16_t*>(out + 8) = (uint16_t)(w1 >> 16);
+                if (i4 == 0) *reinterpret_cast<uint16_t*>(out) = (uint16_t)dbits;
+            }
+        } else {
+            // the sign of m: that of the first value of the lowest lane that has the largest magnitude
+            uint32_t sign = 0;
+#pragma unroll
+            for (int i = 7; i >= 0; i--)
+                if (fabsf(f[i]) == amax) sign = __float_as_uint(f[i]) >> 31;
+            const uint32_t has = __ballot_sync(0xffffffffu, own == amax) >> (threadIdx.x & 28) & 15u;
+            sign = __shfl_sync(0xffffffffu, sign, has ? __ffs(has) - 1 : 0, 4);
+            const float d = amax * (sign ? 0.125f : -0.125f);   // (a power of two: exact but for denormals, where d is 0 in fp16)
+            const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+            uint32_t w0 = 0, w1 = 0;
+#pragma unroll
+            for (int i = 3; i >= 0; i--) {
+                w0 = (w0 << 8) | (nibble_of(f[i], id) & 15u);
+                w1 = (w1 << 8) | (nibble_of(f[4 + i], id) & 15u);
+            }
+            const bool high = i4 & 2;
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? w0 : w1, 2);
+            const uint32_t w = high ? other | (w1 << 4) : w0 | (other << 4);
+            if (!live) return;
+            uint8_t* out = row_out + blk * 18 + 2 + 8 * (i4 & 1) + (high ? 4 : 0);
+            if ((hd & 63) == 0 && (blk & 1)) {
+                *reinterpret_cast<uint32_t*>(out) = w;
+            } else {   // two bytes off a word's boundary
+                *reinterpret_cast<uint16_t*>(out) = (uint16_t)w;
+                *reinterpret_cast<uint16_t*>(out + 2) = (uint16_t)(w >> 16);
+            }
+            if (i4 == 0) *reinterpret_cast<uint16_t*>(row_out + blk * 18) = __half_as_ushort(__float2half_rn(d));
+        }
+    }
+}
+
+// Eight values [c, c + 8) of the cache row at `row`, which a kernel before this one may have written.
+template <int TYPE>
+__device__ __forceinline__ void load_row8(const uint8_t* row, int c, float (&f)[8]) {
+    if constexpr (TYPE == B200_TYPE_F16) {
+        const uint4 u = load_global(reinterpret_cast<const uint4*>(row + 2 * c));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = p.x, f[2 * i + 1] = p.y;
+        }
+    } else {
+        constexpr int BB = TYPE == B200_TYPE_Q8_0 ? 34 : 18;
+        const uint8_t* blk = row + BB * (c >> 5);
+        const float d = __half2float(__ushort_as_half(load_global(reinterpret_cast<const uint16_t*>(blk))));
+        const uint16_t* qs = reinterpret_cast<const uint16_t*>(blk + 2 + (TYPE == B200_TYPE_Q8_0 ? c & 31 : c & 15));
+        const int sh = (c & 16) ? 4 : 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t w = load_global(qs + i);
+            if (TYPE == B200_TYPE_Q8_0) {
+                f[2 * i] = d * (float)(int8_t)(w & 0xFF), f[2 * i + 1] = d * (float)(int8_t)(w >> 8);
+            } else {
+                f[2 * i] = d * (float)((int)(w >> sh & 15u) - 8), f[2 * i + 1] = d * (float)((int)(w >> (8 + sh) & 15u) - 8);
+            }
+        }
+    }
+}
+
+// Eight consecutive values out, rounded to F16 or as they are; V16: 16-byte aligned addresses.
+template <bool F32, bool V16>
+__device__ __forceinline__ void store8(uint8_t* p, const float (&f)[8]) {
+    if constexpr (F32 && V16) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) reinterpret_cast<float*>(p)[i] = f[i];
+    } else if constexpr (V16) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) reinterpret_cast<__half*>(p)[i] = __float2half_rn(f[i]);
+    }
+}
+
+}  // namespace b200

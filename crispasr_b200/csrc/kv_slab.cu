@@ -2,23 +2,14 @@
 //
 // Layout: one arena per cache, holding 2*n_layers slabs (K then V per layer), each slab starting
 // on a 1024-byte boundary.  Inside a slab rows are head-major, ggml view [hd, max_ctx, n_kv, n_streams]:
-//   nb1 = row bytes (hd*2 for F16, hd/32*34 for Q8_0), nb2 = ctx_rows*nb1, nb3 = n_kv*nb2,
+//   nb1 = row bytes (hd*2 for F16, hd/32*34 for Q8_0, hd/32*18 for Q4_0), nb2 = ctx_rows*nb1, nb3 = n_kv*nb2,
 // with ctx_rows = max_ctx rounded up to a multiple of 32 so that every head's row range starts on a
-// 16-byte boundary for both row sizes (a Q8_0 row of head_dim 128 is 136 bytes).
+// 16-byte boundary for all row sizes (a Q8_0 row of head_dim 128 is 136 bytes, a Q4_0 row 72).
 #include <cstdio>
 #include <new>
 
-#include "fattn_common.cuh"
-
-struct b200_kv_cache {
-    b200_kv_config cfg;
-    uint8_t* arena;   // cudaMalloc'ed
-    uint8_t* base;    // arena rounded up to 1024
-    size_t slab_bytes;
-    size_t row_bytes;
-    int64_t ctx_rows;
-    int device;
-};
+#include "kv_cache.h"
+#include "kv_rows.cuh"
 
 namespace b200 {
 namespace {
@@ -48,27 +39,7 @@ __device__ __forceinline__ float4 load4(const uint8_t* p) {
     return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// (int)roundf(t) for |t| < 2^22 without either unit's conversions: |t| + 1/2 truncated to an integer by two additions that
-// round towards zero (the first cannot reach an integer the exact sum does not reach), then the sign; NaN gives 0.  In a block
-// of values below 4e-37 1/d is beyond a float and t infinite: the low byte is that of the saturated conversion, 0xFF for
-// +inf, 0 for -inf (a branch for such blocks cost 0.2 us per launch).
-__device__ __forceinline__ uint32_t round_away(float t) {
-    asm("min.NaN.f32 %0, %0, 0f437F0000;" : "+f"(t));   // 255; a NaN stays one
-    const float m = fmaxf(fabsf(t), 0.0f);
-    const int32_t k = __float_as_int(__fadd_rz(__fadd_rz(m, 0.5f), 8388608.0f)), sign = __float_as_int(t) >> 31;
-    return (uint32_t)((k ^ sign) - sign);
-}
-// Low bytes of four words.
-__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-}
-
-// Q8_0 blocks, bit-identical to gguf-py quantize_blocks: d = amax/127 (fp32), stored as fp16; q = roundf(x * (1/d)) with
-// 1/d = 0 for d == 0.  Four lanes share a block, eight elements each.
-// A block is 34 bytes.  In a row of an even number of blocks (head_dim 64 / 128: rows start on a 4-byte boundary) the
-// quants of the odd blocks fill aligned words and those of the even ones straddle them by two bytes; there a lane takes
-// the upper half of its left neighbour's last word (the first lane the scale) and the row leaves in 32-bit stores.
-template <bool Q8, bool V16, int U>
+template <int TYPE, bool V16, int U>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
     // launched with programmatic stream serialisation: the attention of this layer may set itself up meanwhile; rows are read and
     // written behind the wait, when the previous kernel of the stream has completed
@@ -109,7 +80,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
         }
         // The rows of the next turn into L2 meanwhile: 16 x 407 rows of 8 heads into F16 15.5 -> 14.5 us, 8 x 1500 27.1 -> 26.0.  (Into Q8_0, whose
         // arithmetic covers the loads, 1 %, and the attention behind 8 x 407 rows then starts 0.3 us later.)
-        if (U > 1 && !Q8) {
+        if (U > 1 && TYPE == B200_TYPE_F16) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int row = row0 + (U + u) * step + sub;
@@ -120,50 +91,12 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
         for (int u = 0; u < U; u++) {
             uint8_t* row_out = dst + (int64_t)(row0 + u * step + sub) * a.dnb1;
             const float f[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w, x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
-            if (!Q8) {
-                if (live[u])
-                    *reinterpret_cast<uint4*>(row_out + c * 2) =
-                        make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
-                continue;
-            }
-            float amax = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(f[i]));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const float d = __fdiv_rn(amax, 127.0f);
-            const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-            uint32_t q[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) q[i] = round_away(__fmul_rn(f[i], id));
-            const uint32_t w0 = low_bytes(q[0], q[1], q[2], q[3]), w1 = low_bytes(q[4], q[5], q[6], q[7]);
-            const uint32_t dbits = __half_as_ushort(__float2half_rn(d));
-            const uint32_t left = __shfl_up_sync(0xffffffffu, w1, 1);
-            if (!live[u]) continue;
-            const int blk = c >> 5, i = (c & 31) >> 3;   // lane i of the block's four
-            uint8_t* out = row_out + blk * 34 + 8 * i;
-            if ((a.hd & 63) == 0) {
-                if (blk & 1) {
-                    *reinterpret_cast<uint32_t*>(out + 2) = w0;
-                    *reinterpret_cast<uint32_t*>(out + 6) = w1;
-                    if (i == 0) *reinterpret_cast<uint16_t*>(out) = (uint16_t)dbits;
-                } else {
-                    *reinterpret_cast<uint32_t*>(out) = (w0 << 16) | (i == 0 ? dbits : left >> 16);
-                    *reinterpret_cast<uint32_t*>(out + 4) = __funnelshift_l(w0, w1, 16);
-                    if (i == 3) *reinterpret_cast<uint16_t*>(out + 8) = (uint16_t)(w1 >> 16);
-                }
-            } else {   // an odd number of blocks: rows are only 2-byte aligned
-                *reinterpret_cast<uint16_t*>(out + 2) = (uint16_t)w0;
-                *reinterpret_cast<uint16_t*>(out + 4) = (uint16_t)(w0 >> 16);
-                *reinterpret_cast<uint16_t*>(out + 6) = (uint16_t)w1;
-                *reinterpret_cast<uint16_t*>(out + 8) = (uint16_t)(w1 >> 16);
-                if (i == 0) *reinterpret_cast<uint16_t*>(out) = (uint16_t)dbits;
-            }
+            store_row8<TYPE>(row_out, c, f, live[u], a.hd);
         }
     }
 }
 
-template <bool Q8, bool V16>
+template <int TYPE, bool V16>
 cudaError_t launch_append(AppendArgs a, int n_heads_total, cudaStream_t st) {
     // One token per stream: a warp per (stream, head).  Many rows: eight warps per CTA, four rows (of 128) in flight per warp, and
     // no more CTAs than are resident at once (six per SM), so that a warp's next rows are requested without a new CTA's start.
@@ -181,7 +114,53 @@ cudaError_t launch_append(AppendArgs a, int n_heads_total, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return u == 2 ? cudaLaunchKernelEx(&cfg, kv_append_kernel<Q8, V16, 2>, a) : cudaLaunchKernelEx(&cfg, kv_append_kernel<Q8, V16, 1>, a);
+    return u == 2 ? cudaLaunchKernelEx(&cfg, kv_append_kernel<TYPE, V16, 2>, a) : cudaLaunchKernelEx(&cfg, kv_append_kernel<TYPE, V16, 1>, a);
+}
+
+// Cache rows back to F32 or F16 values: eight per lane, a lane group per row as above.
+struct ReadArgs {
+    const uint8_t* src[2];                   // K, V
+    int64_t snb1, snb2, snb3;
+    uint8_t* dst[2];
+    int64_t dnb1[2], dnb2[2], dnb3[2];
+    int n, hd, n_kv, chunks, ctx_rows, pos0;   // chunks: CTAs per (stream, head)
+    const int32_t* pos;
+};
+
+template <int TYPE, bool F32, bool V16>
+__global__ void __launch_bounds__(256) kv_read_kernel(const ReadArgs a) {
+    let_dependents_launch();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lpr = a.hd / 8, rpw = 32 / lpr, sub = lane / lpr, c = (lane - sub * lpr) * 8;
+    const int which = blockIdx.y, sh = blockIdx.x / a.chunks, chunk = blockIdx.x - sh * a.chunks, s = sh / a.n_kv, h = sh - s * a.n_kv;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (sub >= rpw) return;
+    const int64_t p0 = a.pos ? a.pos[s] : a.pos0;
+    const uint8_t* src = a.src[which] + (int64_t)h * a.snb2 + (int64_t)s * a.snb3;
+    uint8_t* dst = a.dst[which] + (int64_t)h * a.dnb2[which] + (int64_t)s * a.dnb3[which] + (int64_t)c * (F32 ? 4 : 2);
+    for (int row = (chunk * (blockDim.x >> 5) + warp) * rpw + sub; row < a.n; row += a.chunks * (blockDim.x >> 5) * rpw) {
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (p0 + row >= 0 && p0 + row < a.ctx_rows) load_row8<TYPE>(src + (p0 + row) * a.snb1, c, f);
+        store8<F32, V16>(dst + (int64_t)row * a.dnb1[which], f);
+    }
+}
+
+template <int TYPE>
+cudaError_t launch_read(ReadArgs a, int n_heads_total, bool f32, bool v16, cudaStream_t st) {
+    const int rpw = 32 / (a.hd / 8), units = (a.n + rpw - 1) / rpw, per_block = units < 8 ? units : 8;
+    const int full = (units + per_block - 1) / per_block, resident = (148 * 8 + 2 * n_heads_total - 1) / (2 * n_heads_total);
+    a.chunks = full < resident ? full : resident;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.chunks * n_heads_total, 2);
+    cfg.blockDim = dim3(32 * per_block);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (f32) return v16 ? cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, true, true>, a) : cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, true, false>, a);
+    return v16 ? cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, false, true>, a) : cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, false, false>, a);
 }
 
 }  // namespace
@@ -192,13 +171,13 @@ extern "C" {
 B200_API int b200_kv_create(const b200_kv_config* cfg, b200_kv_cache** out) {
     if (!cfg || !out) return B200_E_NULL;
     *out = nullptr;
-    if (cfg->type != B200_TYPE_F16 && cfg->type != B200_TYPE_Q8_0) return B200_E_TYPE;
+    if (cfg->type != B200_TYPE_F16 && cfg->type != B200_TYPE_Q8_0 && cfg->type != B200_TYPE_Q4_0) return B200_E_TYPE;
     if (cfg->head_dim <= 0 || cfg->head_dim % 32 || cfg->head_dim > 128) return B200_E_UNSUPPORTED;
     if (cfg->n_kv_heads <= 0 || cfg->n_layers <= 0 || cfg->max_ctx <= 0 || cfg->n_streams <= 0) return B200_E_SHAPE;
     b200_kv_cache* kv = new (std::nothrow) b200_kv_cache();
     if (!kv) return B200_E_CUDA;
     kv->cfg = *cfg;
-    kv->row_bytes = cfg->type == B200_TYPE_F16 ? (size_t)cfg->head_dim * 2 : (size_t)cfg->head_dim / 32 * 34;
+    kv->row_bytes = b200::kv_row_bytes(cfg->type, cfg->head_dim);
     kv->ctx_rows = ((int64_t)cfg->max_ctx + 31) / 32 * 32;
     const size_t raw = kv->row_bytes * kv->ctx_rows * cfg->n_kv_heads * cfg->n_streams;
     kv->slab_bytes = (raw + 1023) / 1024 * 1024;
@@ -240,7 +219,7 @@ B200_API int b200_kv_view(const b200_kv_cache* kv, int layer, int64_t n_rows, b2
         t->type = kv->cfg.type;
         t->reserved = 0;
         t->ne[0] = kv->cfg.head_dim, t->ne[1] = n_rows, t->ne[2] = kv->cfg.n_kv_heads, t->ne[3] = kv->cfg.n_streams;
-        t->nb[0] = kv->cfg.type == B200_TYPE_F16 ? 2 : 34;
+        t->nb[0] = kv->cfg.type == B200_TYPE_F16 ? 2 : b200::kv_row_bytes(kv->cfg.type, 32);   // an element or a block
         t->nb[1] = kv->row_bytes;
         t->nb[2] = kv->row_bytes * kv->ctx_rows;
         t->nb[3] = t->nb[2] * kv->cfg.n_kv_heads;
@@ -277,9 +256,50 @@ B200_API int b200_kv_append(b200_kv_cache* kv, int layer, const b200_tensor* k_n
     a.ctx_rows = (int)kv->ctx_rows, a.pos = pos, a.pos0 = pos0;
     cudaStream_t st = (cudaStream_t)cuda_stream;
     const int n = kv->cfg.n_kv_heads * kv->cfg.n_streams;
-    const bool q8 = kv->cfg.type == B200_TYPE_Q8_0;
-    const cudaError_t e = q8 ? (v16 ? b200::launch_append<true, true>(a, n, st) : b200::launch_append<true, false>(a, n, st))
-                             : (v16 ? b200::launch_append<false, true>(a, n, st) : b200::launch_append<false, false>(a, n, st));
+    cudaError_t e;
+    switch (kv->cfg.type) {
+        case B200_TYPE_F16: e = v16 ? b200::launch_append<B200_TYPE_F16, true>(a, n, st) : b200::launch_append<B200_TYPE_F16, false>(a, n, st); break;
+        case B200_TYPE_Q8_0: e = v16 ? b200::launch_append<B200_TYPE_Q8_0, true>(a, n, st) : b200::launch_append<B200_TYPE_Q8_0, false>(a, n, st); break;
+        default: e = v16 ? b200::launch_append<B200_TYPE_Q4_0, true>(a, n, st) : b200::launch_append<B200_TYPE_Q4_0, false>(a, n, st); break;
+    }
+    if (e != cudaSuccess || cudaGetLastError() != cudaSuccess) return B200_E_CUDA;
+    return B200_OK;
+}
+
+B200_API int b200_kv_read(const b200_kv_cache* kv, int layer, const b200_tensor* k_out, const b200_tensor* v_out, const int32_t* pos,
+                          int32_t pos0, void* cuda_stream) {
+    if (!kv || !k_out || !v_out) return B200_E_NULL;
+    if (layer < 0 || layer >= kv->cfg.n_layers) return B200_E_SHAPE;
+    b200_tensor view[2];
+    b200_kv_view(kv, layer, kv->ctx_rows, &view[0], &view[1]);
+    b200::ReadArgs a = {};
+    bool v16 = true;
+    for (int which = 0; which < 2; which++) {
+        const b200_tensor* t = which ? v_out : k_out;
+        if (!t->data) return B200_E_NULL;
+        if ((t->type != B200_TYPE_F32 && t->type != B200_TYPE_F16) || t->type != k_out->type) return B200_E_TYPE;
+        const uint64_t es = t->type == B200_TYPE_F32 ? 4 : 2;
+        if (t->nb[0] != es || t->nb[1] % es || t->nb[2] % es || t->nb[3] % es) return B200_E_STRIDE;
+        if ((uintptr_t)t->data % es) return B200_E_ALIGN;
+        if (t->ne[0] != kv->cfg.head_dim || t->ne[2] != kv->cfg.n_kv_heads || t->ne[3] != kv->cfg.n_streams) return B200_E_SHAPE;
+        if (t->ne[1] <= 0 || t->ne[1] > kv->ctx_rows || t->ne[1] != k_out->ne[1]) return B200_E_SHAPE;
+        a.src[which] = (const uint8_t*)view[which].data;
+        a.dst[which] = (uint8_t*)t->data;
+        a.dnb1[which] = (int64_t)t->nb[1], a.dnb2[which] = (int64_t)t->nb[2], a.dnb3[which] = (int64_t)t->nb[3];
+        v16 = v16 && (uintptr_t)t->data % 16 == 0 && t->nb[1] % 16 == 0 && t->nb[2] % 16 == 0 && t->nb[3] % 16 == 0;
+    }
+    a.snb1 = (int64_t)view[0].nb[1], a.snb2 = (int64_t)view[0].nb[2], a.snb3 = (int64_t)view[0].nb[3];
+    a.n = (int)k_out->ne[1], a.hd = kv->cfg.head_dim, a.n_kv = kv->cfg.n_kv_heads, a.ctx_rows = (int)kv->ctx_rows;
+    a.pos = pos, a.pos0 = pos0;
+    const int heads = kv->cfg.n_kv_heads * kv->cfg.n_streams;
+    const bool f32 = k_out->type == B200_TYPE_F32;
+    cudaStream_t st = (cudaStream_t)cuda_stream;
+    cudaError_t e;
+    switch (kv->cfg.type) {
+        case B200_TYPE_F16: e = b200::launch_read<B200_TYPE_F16>(a, heads, f32, v16, st); break;
+        case B200_TYPE_Q8_0: e = b200::launch_read<B200_TYPE_Q8_0>(a, heads, f32, v16, st); break;
+        default: e = b200::launch_read<B200_TYPE_Q4_0>(a, heads, f32, v16, st); break;
+    }
     if (e != cudaSuccess || cudaGetLastError() != cudaSuccess) return B200_E_CUDA;
     return B200_OK;
 }

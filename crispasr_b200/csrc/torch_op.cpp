@@ -11,6 +11,7 @@
 #include <exception>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/CUDADevice.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -110,9 +111,9 @@ bool describe(const at::Tensor& x, long type, b200_tensor* t) {
         PyErr_SetString(PyExc_ValueError, "at most 4 dimensions");
         return false;
     }
-    const bool q8 = type == B200_TYPE_Q8_0;
-    if (q8 && (st != at::kByte || nd == 0 || x.stride(-1) != 1)) {
-        PyErr_SetString(PyExc_ValueError, "Q8_0 tensors are uint8 with a contiguous last axis");
+    const int64_t block = type == B200_TYPE_Q8_0 ? 34 : (type == B200_TYPE_Q4_0 ? 18 : 0);   // bytes of 32 values
+    if (block && (st != at::kByte || nd == 0 || x.stride(-1) != 1)) {
+        PyErr_Format(PyExc_ValueError, "%s tensors are uint8 with a contiguous last axis", block == 34 ? "Q8_0" : "Q4_0");
         return false;
     }
     const int64_t es = x.element_size();
@@ -124,9 +125,9 @@ bool describe(const at::Tensor& x, long type, b200_tensor* t) {
         t->ne[i] = x.size(nd - 1 - i);
         t->nb[i] = (uint64_t)(x.stride(nd - 1 - i) * es);
     }
-    if (q8) t->ne[0] = t->ne[0] / 34 * 32, t->nb[0] = 34;
+    if (block) t->ne[0] = t->ne[0] / block * 32, t->nb[0] = (uint64_t)block;
     if (nd == 0) t->nb[0] = (uint64_t)es;
-    for (int i = nd > 1 ? nd : 1; i < 4; i++) t->nb[i] = t->nb[i - 1] * (uint64_t)(q8 && i == 1 ? t->ne[0] / 32 : t->ne[i - 1]);
+    for (int i = nd > 1 ? nd : 1; i < 4; i++) t->nb[i] = t->nb[i - 1] * (uint64_t)(block && i == 1 ? t->ne[0] / 32 : t->ne[i - 1]);
     return true;
 }
 
@@ -391,10 +392,307 @@ PyObject* kv_append_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- norm, rotation and append; reading rows back ----------------------------------------------------------------------------
+
+// The arguments of the rotation's calls; all by keyword, unknown names are an error.
+enum RopeKey { rQNorm, rKNorm, rEps, rDims, rBase, rScale, rNeox, rPos, rPos0, rNRows, rOut, rKOut, rStream, rKeys };
+const char* const kRopeNames[rKeys] = {"q_norm", "k_norm", "eps", "rope_dims", "rope_base", "rope_scale", "neox", "pos", "pos0", "n_rows", "out", "k_out", "stream"};
+PyObject* g_rope_keys[rKeys];
+
+// An int32 table on the device of `like`, one entry per stream.
+bool table_of(PyObject* o, const char* what, const at::Tensor& like, int64_t streams, const int32_t** out) {
+    const at::Tensor* t = tensor_of(o, what);
+    if (!t) return false;
+    if (t->scalar_type() != at::kInt || t->device() != like.device() || t->numel() != streams || !t->is_contiguous()) {
+        PyErr_Format(PyExc_ValueError, "%s is a contiguous int32 tensor of %lld entries on the rows' device", what, (long long)streams);
+        return false;
+    }
+    *out = (const int32_t*)t->data_ptr();
+    return true;
+}
+
+bool rows_of(PyObject* o, const char* what, const at::Tensor* like, const at::Tensor** out) {
+    const at::Tensor* t = tensor_of(o, what);
+    if (!t) return false;
+    if (!t->is_cuda() || (like && t->device() != like->device())) {
+        PyErr_Format(PyExc_ValueError, like ? "%s is on another device than the other rows" : "%s is a CUDA tensor", what);
+        return false;
+    }
+    if (t->dim() != 4) {
+        PyErr_Format(PyExc_ValueError, "%s is (streams, heads, rows, head_dim)", what);
+        return false;
+    }
+    *out = t;
+    return true;
+}
+
+struct RopeCall {
+    PyObject* v[rKeys] = {};   // borrowed
+    b200_rope_params params{0, B200_ROPE_NEOX, 10000.0f, 1.0f, 1e-6f, 0};
+    b200_tensor norm[2];
+    const b200_tensor* norm_p[2] = {nullptr, nullptr};
+    const int32_t *pos = nullptr, *n_rows = nullptr;
+    int32_t pos0 = 0;
+    void* stream = nullptr;
+
+    bool parse(PyObject* names, PyObject* const* values, const char* where) {
+        const Py_ssize_t n = names ? PyTuple_GET_SIZE(names) : 0;
+        for (Py_ssize_t j = 0; j < n; j++) {
+            PyObject* name = PyTuple_GET_ITEM(names, j);
+            int hit = -1;
+            for (int i = 0; i < rKeys && hit < 0; i++)
+                if (name == g_rope_keys[i]) hit = i;
+            for (int i = 0; i < rKeys && hit < 0; i++)
+                if (PyUnicode_Compare(name, g_rope_keys[i]) == 0) hit = i;
+            if (PyErr_Occurred()) return false;
+            if (hit < 0) {
+                PyErr_Format(PyExc_TypeError, "%s() got an unexpected keyword argument '%U'", where, name);
+                return false;
+            }
+            v[hit] = values[j] == Py_None ? nullptr : values[j];
+        }
+        return true;
+    }
+    bool number(RopeKey k, float* out) const {
+        if (!v[k]) return true;
+        const double d = PyFloat_AsDouble(v[k]);
+        if (d == -1.0 && PyErr_Occurred()) return false;
+        *out = (float)d;
+        return true;
+    }
+    bool integer(RopeKey k, int32_t* out) const {
+        if (!v[k]) return true;
+        const long i = PyLong_AsLong(v[k]);
+        if (i == -1 && PyErr_Occurred()) return false;
+        if (i != (int32_t)i) {
+            PyErr_Format(PyExc_OverflowError, "%s is a 32-bit number", kRopeNames[k]);
+            return false;
+        }
+        *out = (int32_t)i;
+        return true;
+    }
+    // What the call says beside its rows; `like`: (streams, heads, rows, head_dim).
+    bool fill(const at::Tensor& like) {
+        params.n_dims = (int32_t)like.size(3);
+        if (!number(rEps, &params.eps) || !number(rBase, &params.freq_base) || !number(rScale, &params.freq_scale) || !integer(rDims, &params.n_dims) ||
+            !integer(rPos0, &pos0))
+            return false;
+        if (v[rNeox]) {
+            const int t = PyObject_IsTrue(v[rNeox]);
+            if (t < 0) return false;
+            params.mode = t ? B200_ROPE_NEOX : B200_ROPE_NORM;
+        }
+        for (int x = 0; x < 2; x++) {
+            const RopeKey key = x ? rKNorm : rQNorm;
+            if (!v[key]) continue;
+            const at::Tensor* w = tensor_of(v[key], kRopeNames[key]);
+            if (!w) return false;
+            if (w->device() != like.device()) {
+                PyErr_Format(PyExc_ValueError, "%s is on another device than the rows", kRopeNames[key]);
+                return false;
+            }
+            if (!describe(*w, -1, &norm[x])) return false;
+            norm_p[x] = &norm[x];
+        }
+        if (v[rPos] && !table_of(v[rPos], "pos", like, like.size(0), &pos)) return false;
+        if (v[rNRows] && !table_of(v[rNRows], "n_rows", like, like.size(0), &n_rows)) return false;
+        if (!v[rStream]) stream = c10::cuda::getCurrentCUDAStream(like.device().index()).stream();
+        else if (!stream_of(v[rStream], &stream)) return false;
+        return true;
+    }
+    // The rows that a call writes: given, or made here.
+    const at::Tensor* output(RopeKey k, const at::Tensor& like, at::ScalarType type, at::Tensor* made) const {
+        const at::Tensor* out = made;
+        if (!v[k]) *made = at::detail::empty_cuda(like.sizes(), type, like.device(), std::nullopt);
+        else if (!rows_of(v[k], kRopeNames[k], &like, &out)) return nullptr;
+        return out;
+    }
+};
+
+const char kQkRopeDoc[] =
+    "qk_norm_rope(q, k=None, *, q_norm=None, k_norm=None, eps=1e-6, rope_dims=head_dim, rope_base=10000.0, rope_scale=1.0, neox=True,\n"
+    "             pos=None, pos0=0, n_rows=None, out=None, k_out=None, stream=None)\n--\n\n"
+    "Norm of every head (where a weight is given) and rotation by position of q (streams, heads, rows, head_dim) and k (streams,\n"
+    "kv heads, rows, head_dim), F32 or F16: (rotated q, rotated k or None), of q's type unless `out` and `k_out` say otherwise (they may\n"
+    "be q and k).  Row i of stream s is at position pos[s] + i (`pos` an int32 CUDA tensor, else `pos0` for all); rows at or\n"
+    "beyond n_rows[s] (an int32 CUDA tensor) are zeros.  Asynchronous on `stream` (default: torch's current stream).";
+
+PyObject* qk_norm_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObject* names) {
+    HANDLE_TH_ERRORS
+    if (n < 1 || n > 2) {
+        PyErr_SetString(PyExc_TypeError, "qk_norm_rope() takes 1 or 2 positional arguments (q, k)");
+        return nullptr;
+    }
+    RopeCall call;
+    const at::Tensor *q = nullptr, *k = nullptr;
+    if (!call.parse(names, a + n, "qk_norm_rope") || !rows_of(a[0], "q", nullptr, &q)) return nullptr;
+    if (n > 1 && a[1] != Py_None && !rows_of(a[1], "k", q, &k)) return nullptr;
+    if (!k && call.v[rKOut]) {
+        PyErr_SetString(PyExc_ValueError, "k_out without k");
+        return nullptr;
+    }
+    const c10::cuda::CUDAGuard guard(q->device());
+    if (!call.fill(*q)) return nullptr;
+    b200_tensor tq, tk, to, tko;
+    at::Tensor made, made_k;
+    const at::Tensor *out = nullptr, *k_out = nullptr;
+    if (!describe(*q, -1, &tq) || (k && !describe(*k, -1, &tk)) || !(out = call.output(rOut, *q, q->scalar_type(), &made)) || !describe(*out, -1, &to)) return nullptr;
+    if (k && (!(k_out = call.output(rKOut, *k, out->scalar_type(), &made_k)) || !describe(*k_out, -1, &tko))) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = b200_qk_norm_rope(&tq, k ? &tk : nullptr, call.norm_p[0], call.norm_p[1], &call.params, call.pos, call.pos0, call.n_rows, &to, k ? &tko : nullptr, call.stream);
+    Py_END_ALLOW_THREADS
+    if (rc) return raise_code(rc, "b200_qk_norm_rope");
+    PyObject* first = THPVariable_Wrap(*out);
+    PyObject* second = k ? THPVariable_Wrap(*k_out) : Py_NewRef(Py_None);
+    PyObject* both = first && second ? PyTuple_Pack(2, first, second) : nullptr;
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// (cache address, layer, q, k_new, v_new, *, ...)
+PyObject* kv_append_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObject* names) {
+    HANDLE_TH_ERRORS
+    if (n != 5) {
+        PyErr_SetString(PyExc_TypeError, "append_rope() takes 4 positional arguments (layer, q, k_new, v_new)");
+        return nullptr;
+    }
+    b200_kv_cache* kv = (b200_kv_cache*)PyLong_AsVoidPtr(a[0]);
+    const long layer = PyLong_AsLong(a[1]);
+    if (PyErr_Occurred()) return nullptr;
+    RopeCall call;
+    const at::Tensor *q = nullptr, *k = nullptr, *v = nullptr;
+    if (!call.parse(names, a + n, "append_rope") || !rows_of(a[3], "k_new", nullptr, &k) || !rows_of(a[4], "v_new", k, &v)) return nullptr;
+    if (a[2] != Py_None && !rows_of(a[2], "q", k, &q)) return nullptr;
+    if (call.v[rKOut] || (!q && call.v[rOut])) {
+        PyErr_SetString(PyExc_TypeError, call.v[rKOut] ? "append_rope() has no k_out: k goes into the cache" : "append_rope() got out without q");
+        return nullptr;
+    }
+    const c10::cuda::CUDAGuard guard(k->device());
+    if (!call.fill(*k)) return nullptr;
+    b200_tensor tq, tk, tv, to;
+    at::Tensor made;
+    const at::Tensor* out = nullptr;
+    if (!describe(*k, -1, &tk) || !describe(*v, -1, &tv)) return nullptr;
+    if (q && (!describe(*q, -1, &tq) || !(out = call.output(rOut, *q, at::kHalf, &made)) || !describe(*out, -1, &to))) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = b200_kv_append_rope(kv, (int)layer, q ? &tq : nullptr, &tk, &tv, call.norm_p[0], call.norm_p[1], &call.params, call.pos, call.pos0, call.n_rows,
+                             q ? &to : nullptr, call.stream);
+    Py_END_ALLOW_THREADS
+    if (rc) return raise_code(rc, "b200_kv_append_rope");
+    if (!q) Py_RETURN_NONE;
+    return THPVariable_Wrap(*out);
+    END_HANDLE_TH_ERRORS
+}
+
+int device_of_cache(const void* p) { return at::cuda::getDeviceFromPtr(const_cast<void*>(p)).index(); }
+
+// (cache address, cache object, layer, n_rows): the views of kv_view as torch tensors that keep the cache object alive
+PyObject* kv_tensors_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 4) {
+        PyErr_SetString(PyExc_TypeError, "kv_tensors takes 4 arguments");
+        return nullptr;
+    }
+    HANDLE_TH_ERRORS
+    const b200_kv_cache* kv = (const b200_kv_cache*)PyLong_AsVoidPtr(a[0]);
+    const long layer = PyLong_AsLong(a[2]), rows = PyLong_AsLong(a[3]);
+    if (PyErr_Occurred()) return nullptr;
+    b200_tensor t[2];
+    const int rc = b200_kv_view(kv, (int)layer, rows, &t[0], &t[1]);
+    if (rc) return raise_code(rc, "b200_kv_view");
+    PyObject* views[2];
+    for (int i = 0; i < 2; i++) {
+        const bool f16 = t[i].type == B200_TYPE_F16;
+        const int64_t es = f16 ? 2 : 1, width = f16 ? t[i].ne[0] : t[i].ne[0] / 32 * (int64_t)t[i].nb[0];
+        const int64_t sizes[4] = {t[i].ne[3], t[i].ne[2], t[i].ne[1], width};
+        const int64_t strides[4] = {(int64_t)t[i].nb[3] / es, (int64_t)t[i].nb[2] / es, (int64_t)t[i].nb[1] / es, 1};
+        PyObject* owner = Py_NewRef(a[1]);
+        views[i] = THPVariable_Wrap(at::from_blob(
+            t[i].data, sizes, strides,
+            [owner](void*) {
+                if (!Py_IsInitialized()) return;
+                const PyGILState_STATE gil = PyGILState_Ensure();
+                Py_DECREF(owner);
+                PyGILState_Release(gil);
+            },
+            at::TensorOptions().dtype(f16 ? at::kHalf : at::kByte).device(at::kCUDA, (c10::DeviceIndex)device_of_cache(t[i].data))));
+    }
+    PyObject* both = views[0] && views[1] ? PyTuple_Pack(2, views[0], views[1]) : nullptr;
+    Py_XDECREF(views[0]);
+    Py_XDECREF(views[1]);
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// (cache address, layer, n_rows, pos, pos0, f32, out, stream): K and V rows as values
+PyObject* kv_read_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 8) {
+        PyErr_SetString(PyExc_TypeError, "kv_read takes 8 arguments");
+        return nullptr;
+    }
+    HANDLE_TH_ERRORS
+    const b200_kv_cache* kv = (const b200_kv_cache*)PyLong_AsVoidPtr(a[0]);
+    const long layer = PyLong_AsLong(a[1]), rows = PyLong_AsLong(a[2]), pos0 = PyLong_AsLong(a[4]);
+    const int f32 = PyObject_IsTrue(a[5]);
+    if (PyErr_Occurred()) return nullptr;
+    if (pos0 != (int32_t)pos0) {
+        PyErr_SetString(PyExc_OverflowError, "pos0 is a 32-bit number");
+        return nullptr;
+    }
+    b200_tensor view[2], t[2];
+    int rc = b200_kv_view(kv, (int)layer, rows, &view[0], &view[1]);
+    if (rc) return raise_code(rc, "b200_kv_view");
+    const c10::Device device(at::kCUDA, (c10::DeviceIndex)device_of_cache(view[0].data));
+    const c10::cuda::CUDAGuard guard(device);
+    const int64_t sizes[4] = {view[0].ne[3], view[0].ne[2], rows, view[0].ne[0]};
+    at::Tensor out[2];
+    if (a[6] == Py_None) {
+        for (at::Tensor& o : out) o = at::detail::empty_cuda(sizes, f32 ? at::kFloat : at::kHalf, device, std::nullopt);
+    } else {
+        if (!PyTuple_Check(a[6]) || PyTuple_GET_SIZE(a[6]) != 2) {
+            PyErr_SetString(PyExc_TypeError, "out is a pair of tensors");
+            return nullptr;
+        }
+        for (int i = 0; i < 2; i++) {
+            const at::Tensor* o = nullptr;
+            if (!rows_of(PyTuple_GET_ITEM(a[6], i), "out", nullptr, &o)) return nullptr;
+            if (o->device() != device || o->size(2) != rows) {
+                PyErr_SetString(PyExc_ValueError, "out has n_rows rows and is on the cache's device");
+                return nullptr;
+            }
+            out[i] = *o;
+        }
+    }
+    if (!describe(out[0], -1, &t[0]) || !describe(out[1], -1, &t[1])) return nullptr;
+    const int32_t* pos = nullptr;
+    if (a[3] != Py_None && !table_of(a[3], "pos", out[0], sizes[0], &pos)) return nullptr;
+    void* st = nullptr;
+    if (a[7] == Py_None) st = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    else if (!stream_of(a[7], &st)) return nullptr;
+    Py_BEGIN_ALLOW_THREADS
+    rc = b200_kv_read(kv, (int)layer, &t[0], &t[1], pos, (int32_t)pos0, st);
+    Py_END_ALLOW_THREADS
+    if (rc) return raise_code(rc, "b200_kv_read");
+    PyObject* first = THPVariable_Wrap(out[0]);
+    PyObject* second = THPVariable_Wrap(out[1]);
+    PyObject* both = first && second ? PyTuple_Pack(2, first, second) : nullptr;
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"flash_attn_ext", (PyCFunction)(void (*)(void))launch_py, METH_FASTCALL | METH_KEYWORDS, kLaunchDoc},
     {"flash_attn_ext_host", (PyCFunction)(void (*)(void))forward_host_py, METH_FASTCALL | METH_KEYWORDS, kHostDoc},
     {"kv_append", (PyCFunction)(void (*)(void))kv_append_py, METH_FASTCALL, "rows of a KV cache"},
+    {"qk_norm_rope", (PyCFunction)(void (*)(void))qk_norm_rope_py, METH_FASTCALL | METH_KEYWORDS, kQkRopeDoc},
+    {"kv_append_rope", (PyCFunction)(void (*)(void))kv_append_rope_py, METH_FASTCALL | METH_KEYWORDS, "norm, rotation and rows of a KV cache"},
+    {"kv_tensors", (PyCFunction)(void (*)(void))kv_tensors_py, METH_FASTCALL, "views of a KV cache"},
+    {"kv_read", (PyCFunction)(void (*)(void))kv_read_py, METH_FASTCALL, "rows of a KV cache as values"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_op", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
@@ -403,5 +701,7 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_op", nullptr, -1, kMethods
 PyMODINIT_FUNC PyInit__torch_op(void) {
     for (int i = 0; i < kKeys; i++)
         if (!(g_keys[i] = PyUnicode_InternFromString(kKeyNames[i]))) return nullptr;
+    for (int i = 0; i < rKeys; i++)
+        if (!(g_rope_keys[i] = PyUnicode_InternFromString(kRopeNames[i]))) return nullptr;
     return PyModule_Create(&kModule);
 }

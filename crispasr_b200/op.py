@@ -2,7 +2,7 @@
 logit_softcap) (reference call sites: src/crispasr.cpp:2821, src/core/attention.h:992).
 
 Tensors are torch tensors in torch order (slowest first): q (B,H,Tq,hd), k/v (Bk,Hkv,Lk,hd) or uint8
-Q8_0 block rows (Bk,Hkv,Lk,hd/32*34), mask (1|B,1|H,Tq,Lk) f16; the result is (B,Tq,H,hd) f32, i.e.
+block rows (Q8_0: (Bk,Hkv,Lk,hd/32*34), Q4_0: (Bk,Hkv,Lk,hd/32*18), named by kv_type), mask (1|B,1|H,Tq,Lk) f16; the result is (B,Tq,H,hd) f32, i.e.
 ggml's dst [hd,H,Tq,B].  Any of them may be a strided view.
 """
 from __future__ import annotations
@@ -104,7 +104,8 @@ def workspace_bytes(q, k, v, mask=None, **kw) -> int:
 # The torch-facing call path is native code (csrc/torch_op.cpp): a decode step is a row of calls of a few microseconds each,
 # and a wrapper in Python would cost a tenth of them.  It links against torch, which is imported with the first use of one
 # of its functions: the rest of the package needs none.
-_NATIVE = {"flash_attn_ext": "flash_attn_ext", "flash_attn_ext_host": "flash_attn_ext_host", "_kv_append": "kv_append"}
+_NATIVE = {"flash_attn_ext": "flash_attn_ext", "flash_attn_ext_host": "flash_attn_ext_host", "qk_norm_rope": "qk_norm_rope", "_kv_append": "kv_append",
+           "_kv_append_rope": "kv_append_rope", "_kv_tensors": "kv_tensors", "_kv_read": "kv_read"}
 
 
 def _load_native():
@@ -167,6 +168,34 @@ class KvCache:
         if "_kv_append" not in globals():
             _load_native()
         _kv_append(self._h.value or 0, layer, k_new, v_new, pos, pos0, stream)  # noqa: F821
+
+    def append_rope(self, layer, q, k_new, v_new, **kw):
+        """b200_kv_append_rope: norm (where a weight is given) and rotation of q (n_streams, heads, n_new, hd; or None) and
+        k_new (n_streams, n_kv, n_new, hd), and k_new and v_new into the cache.  All float32 or all float16 CUDA tensors.
+        Keywords as in :func:`qk_norm_rope` (q_norm, k_norm, eps, rope_dims, rope_base, rope_scale, neox, pos, pos0, n_rows, out,
+        stream); the position of a row is its place in the cache.  Returns the rotated q, float16 unless `out` says otherwise."""
+        if "_kv_append_rope" not in globals():
+            _load_native()
+        return _kv_append_rope(self._h.value or 0, layer, q, k_new, v_new, **kw)  # noqa: F821
+
+    def tensors(self, layer, n_rows):
+        """Rows [0, n_rows) of a layer as torch tensors on the cache's memory: (K, V), each (n_streams, n_kv, n_rows, hd) float16 or
+        (n_streams, n_kv, n_rows, bytes of a row) uint8 blocks, as flash_attn_ext takes them.  They keep this object alive; after
+        close() they must not be used."""
+        if "_kv_tensors" not in globals():
+            _load_native()
+        return _kv_tensors(self._h.value or 0, self, layer, n_rows)  # noqa: F821
+
+    def read(self, layer, n_rows, pos=None, pos0=0, dtype=None, out=None, stream=None):
+        """b200_kv_read: rows pos[s] .. pos[s] + n_rows - 1 of every stream (`pos` an int32 CUDA tensor, else `pos0` for all) as values:
+        (K, V), each (n_streams, n_kv, n_rows, hd) float16, or float32 if `dtype` says so, or the pair `out`.  Rows outside
+        the cache are zeros."""
+        if "_kv_read" not in globals():
+            _load_native()
+        import torch
+        if dtype not in (None, torch.float16, torch.float32):
+            raise ValueError("dtype is torch.float16 or torch.float32")
+        return _kv_read(self._h.value or 0, layer, n_rows, pos, pos0, dtype is torch.float32, out, stream)  # noqa: F821
 
     def copy_stream(self, dst_stream, src_stream, n_rows, stream=None):
         """Fork a hypothesis: rows [0, n_rows) of every layer/head from one stream to another (kv_snapshot_pool)."""

@@ -1,10 +1,11 @@
 /*
  * b200_fattn.h — C-ABI of the B200-native fused attention path.
  *
- * This library implements exactly one operator of the CrispASR/ggml stack,
- * GGML_OP_FLASH_ATTN_EXT, plus the two pieces of host plumbing that feed it
- * (a KV-cache slab allocator and a per-GPU segment scheduler).  Every entry
- * point is plain C: pointers, sizes and enums, no C++ or torch types.
+ * This library implements the attention operator of the CrispASR/ggml stack,
+ * GGML_OP_FLASH_ATTN_EXT, the KV cache that feeds it with the pass that fills
+ * it (norm and rotation of Q and K, append), and a per-GPU segment scheduler.
+ * Every entry point is plain C: pointers, sizes and enums, no C++ or torch
+ * types.
  *
  * Tensor descriptors use ggml conventions throughout: ne[0] is the fastest
  * dimension, nb[i] is the stride of dimension i in BYTES, nb[0] is the size of
@@ -16,7 +17,7 @@
  * src/core/cross_attn.h:148; src/canary.cpp:971,994):
  *
  *   Q    [hd,  Tq, H,   B]  F32 or F16, nb[0] == element size
- *   K    [hd,  Lk, Hkv, Bk] F16, F32 or Q8_0 (34-byte blocks of 32), H % Hkv == 0, B % Bk == 0
+ *   K    [hd,  Lk, Hkv, Bk] F16, F32, Q8_0 (34-byte blocks of 32) or Q4_0 (18-byte blocks of 32), H % Hkv == 0, B % Bk == 0
  *   V    [hdv, Lk, Hkv, Bk] same type as K (hdv == hd in this library)
  *   mask [Lk,  Tq, 1|H, 1|B] F16 or NULL; 0 = attend, -inf = masked, any finite value = additive bias
  *   dst  [hdv, H,  Tq,  B]  F32, contiguous; 16-byte aligned base for head_dim 64 / 128 (else B200_E_ALIGN)
@@ -27,8 +28,9 @@
  *   dst[:,h,q,b] = sum_k softmax_k(s)[k] * V[:,k,...]      (fp32 softmax, fp32 accumulation)
  *
  * Q is rounded to F16 before the dot product (it is the tensor-core operand
- * type); K/V quantised blocks are dequantised as fp32(d) * q.  A row whose keys
- * are all masked yields zeros.
+ * type); K/V quantised blocks are dequantised as fp32(d) * q (Q8_0) or
+ * fp32(d) * (q - 8) (Q4_0: value i of a block in the low nibble of byte i,
+ * value 16 + i in the high one).  A row whose keys are all masked yields zeros.
  */
 #ifndef B200_FATTN_H
 #define B200_FATTN_H
@@ -46,10 +48,11 @@ extern "C" {
 #define B200_API __attribute__((visibility("default")))
 #endif
 
-/* Numeric ids equal ggml's GGML_TYPE_* / gguf-py GGMLQuantizationType (F32=0, F16=1, Q8_0=8). */
+/* Numeric ids equal ggml's GGML_TYPE_* / gguf-py GGMLQuantizationType (F32=0, F16=1, Q4_0=2, Q8_0=8). */
 typedef enum b200_type {
     B200_TYPE_F32 = 0,
     B200_TYPE_F16 = 1,
+    B200_TYPE_Q4_0 = 2,
     B200_TYPE_Q8_0 = 8,
 } b200_type;
 
@@ -303,12 +306,12 @@ B200_API int b200_last_kernel(void);
  * src/core/attention.h:593-595) and whisper's kv_self / kv_cross buffers
  * (src/crispasr.cpp:1471-1516): one contiguous, 1024-byte aligned slab per layer and per K/V,
  * head-major rows, so that every (layer, kv-head) row range is a single flat byte range that
- * TMA boxes (F16) or 128-bit streaming loads (Q8_0) can cover.
+ * TMA boxes (F16) or bulk copies of whole tiles (Q8_0, Q4_0) can cover.
  * ------------------------------------------------------------------------------------------ */
 typedef struct b200_kv_cache b200_kv_cache; /* opaque */
 
 typedef struct b200_kv_config {
-    int32_t type;     /* B200_TYPE_F16 or B200_TYPE_Q8_0 */
+    int32_t type;     /* B200_TYPE_F16, B200_TYPE_Q8_0 or B200_TYPE_Q4_0 */
     int32_t head_dim; /* 64 or 128 (multiple of 32) */
     int32_t n_kv_heads;
     int32_t n_layers;
@@ -332,6 +335,57 @@ B200_API int b200_kv_view(const b200_kv_cache* kv, int layer, int64_t n_rows, b2
  */
 B200_API int b200_kv_append(b200_kv_cache* kv, int layer, const b200_tensor* k_new, const b200_tensor* v_new,
                             const int32_t* pos, int32_t pos0, void* cuda_stream);
+/*
+ * b200_kv_read — rows of the cache as the values they stand for: replaces the view + ggml_cast(F32) with which the
+ * runtimes read a quantised cache (src/core/attention.h:887-920), for callers that move a stream to a cache of another
+ * type, keep it on the host or feed an operator of their own.  k_out/v_out are F32 or F16 (both the same)
+ * [hd, n, n_kv_heads, n_streams] on the device, generic strides; row i of stream s is cache row pos[s] + i (`pos0` + i where
+ * `pos` is NULL), rows outside the cache read as zeros.  Asynchronous on `cuda_stream`.
+ */
+B200_API int b200_kv_read(const b200_kv_cache* kv, int layer, const b200_tensor* k_out, const b200_tensor* v_out,
+                          const int32_t* pos, int32_t pos0, void* cuda_stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The pass between the projections of a decoder layer and its attention: the norm of every query and key head
+ * (ggml_rms_norm + ggml_mul of the Qwen-style runtimes, src/qwen3_asr.cpp:1242-1277), the rotation by position
+ * (ggml_rope_ext, src/core/attention.h:725-822), and the new rows' way into the cache (:840-867), five to eight
+ * graph nodes, as one launch that reads every row once.  For a row x of a head at position p:
+ *   y = x * weight / sqrt(mean(x^2) + eps)                            (without a weight: y = x)
+ *   (y[a], y[b]) <- (y[a] cos t - y[b] sin t, y[a] sin t + y[b] cos t),  t = p * freq_scale * freq_base^(-2 i / n_dims)
+ * for every pair i < n_dims / 2: (a, b) = (i, i + n_dims/2) with B200_ROPE_NEOX, (2i, 2i + 1) with B200_ROPE_NORM; values
+ * n_dims.. of a head are not rotated.  Angles are reduced exactly (64-bit fixed point), sums and products are fp32, and
+ * the result is rounded once to its type.
+ * ------------------------------------------------------------------------------------------ */
+enum { B200_ROPE_NORM = 0, B200_ROPE_NEOX = 2 };   /* ggml's GGML_ROPE_TYPE_NORMAL / _NEOX */
+typedef struct b200_rope_params {
+    int32_t n_dims;    /* rotated values of a head: even, at most head_dim (NEOX: a multiple of 16, else B200_E_UNSUPPORTED); 0 = no rotation */
+    int32_t mode;      /* B200_ROPE_NORM or B200_ROPE_NEOX */
+    float freq_base;   /* > 0 */
+    float freq_scale;
+    float eps;         /* of the norm, >= 0 */
+    int32_t reserved;
+} b200_rope_params;
+/*
+ * b200_qk_norm_rope — norm and rotation alone, for callers with caches of their own.  q [hd, n, H, S] and k [hd, n, Hkv, S]
+ * (k and k_out may be NULL) are F32 or F16 (both the same), device, generic strides, hd a multiple of 8 up to 128; q_out and
+ * k_out have their shapes and are F32 or F16 (both the same); an output may be its input.  q_norm / k_norm: F32 [hd] weights,
+ * or NULL (no norm).  Row i of stream s is at position pos[s] + i (`pos` a device array [S], or NULL meaning `pos0` for all).
+ * n_rows: device array [S] of valid rows per stream, or NULL; output rows at or beyond it are zeros.  Asynchronous on
+ * `cuda_stream`.
+ */
+B200_API int b200_qk_norm_rope(const b200_tensor* q, const b200_tensor* k, const b200_tensor* q_norm, const b200_tensor* k_norm,
+                               const b200_rope_params* params, const int32_t* pos, int32_t pos0, const int32_t* n_rows,
+                               const b200_tensor* q_out, const b200_tensor* k_out, void* cuda_stream);
+/*
+ * b200_kv_append_rope — the same for q (to q_out; both may be NULL) and k_new, and k_new and v_new converted to the cache
+ * type and stored at rows pos[s] .. of every stream, as b200_kv_append stores them; the position of a row is its place in
+ * the cache.  q, k_new and v_new are all F32 or all F16.  Rows at or beyond n_rows[s], and rows outside the cache, are not
+ * stored.
+ */
+B200_API int b200_kv_append_rope(b200_kv_cache* kv, int layer, const b200_tensor* q, const b200_tensor* k_new, const b200_tensor* v_new,
+                                 const b200_tensor* q_norm, const b200_tensor* k_norm, const b200_rope_params* params,
+                                 const int32_t* pos, int32_t pos0, const int32_t* n_rows, const b200_tensor* q_out,
+                                 void* cuda_stream);
 
 /*
  * b200_kv_copy_stream — replaces core_attn::kv_snapshot_pool save/restore (src/core/attention.h:198-320), the
