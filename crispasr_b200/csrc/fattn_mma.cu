@@ -423,7 +423,8 @@ enum DecodeMode {
     kDecSync = 0,    // element loads + conversion (F32 K/V, unaligned or gapped layouts)
     kDecAsyncF16 = 1,  // cp.async 16-byte copies of F16 rows into a multi-stage ring
     kDecAsyncQ8 = 2,   // bulk copy of the raw Q8_0 byte range of a tile, then a shared-to-shared dequantise (head_dim 32)
-    kDecRegQ8 = 3      // bulk copy of the raw Q8_0 bytes, dequantised in registers (head_dim 64 / 128)
+    kDecRegQ8 = 3,     // bulk copy of the raw Q8_0 bytes, dequantised in registers (head_dim 64 / 128)
+    kDecRegQ4 = 4      // the same over a Q4_0 cache (head_dim 64 / 128, at most 8 query rows, no mask, no softcap)
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -670,7 +671,8 @@ __host__ __device__ constexpr size_t cluster_push_bytes(int hd, int rows) { retu
 // A CTA with two or three tiles shares its SM with few others, but at the usual 256-stream size three neighbours are
 // in their key loops and every dependent step of a tail waits for an issue slot, so the chain is kept short: no
 // separate pass for the common maximum, no index division per element.
-template <int HD, int NW = 4, int ROWS = kDecRows>
+// PAIR: a query row's partial is the sum of slab rows rr and rr + 4.
+template <int HD, int NW = 4, int ROWS = kDecRows, bool PAIR = false>
 __device__ __forceinline__ void decode_write_out(const FattnArgs& a, const float* slab, const float (*s_m)[kDecRows],
                                                  const float (*s_l)[kDecRows], uint8_t* recv, int R, int b, int hk, int split,
                                                  int tq_b, int tid) {
@@ -686,7 +688,13 @@ __device__ __forceinline__ void decode_write_out(const FattnArgs& a, const float
         float m[NW], w[NW], M = ninf, L = 0.0f;
         float4 x[NW], v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < NW; i++) m[i] = s_m[i][rr], x[i] = *reinterpret_cast<const float4*>(slab + (i * ROWS + rr) * STRIDE + 4 * cg);
+        for (int i = 0; i < NW; i++) {
+            m[i] = s_m[i][rr], x[i] = *reinterpret_cast<const float4*>(slab + (i * ROWS + rr) * STRIDE + 4 * cg);
+            if (PAIR) {
+                const float4 y = *reinterpret_cast<const float4*>(slab + (i * ROWS + rr + 4) * STRIDE + 4 * cg);
+                x[i].x += y.x, x[i].y += y.y, x[i].z += y.z, x[i].w += y.w;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < NW; i++) M = fmaxf(M, m[i]);
 #pragma unroll
@@ -1758,6 +1766,8 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q8t_kernel(cons
     decode_write_out<HD, NW, 8>(a, slab, s_m, s_l, sRaw + NS * 2 * RAW_BYTES, R, b, hk, split, tq_b, tid);
 }
 
+#include "fattn_decode_q4.cuh"
+
 // One warp per (batch, kv-head, row): log-sum-exp merge of the split partials.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) fattn_merge_kernel(const FattnArgs a) {
@@ -1992,8 +2002,16 @@ int decode_mode(const FattnArgs& a, int hdp) {
         if (!a.kv_index && contiguous_rows && aligned && tail_ok && a.v.nb2 >= ((int64_t)a.Lk * rb + 15) / 16 * 16)   // gathered rows are not contiguous: element path
             return (a.hd == 64 || a.hd == 128) ? kDecRegQ8 : kDecAsyncQ8;
     }
+    // Q4_0: rows that follow one another, from any 4-byte boundary on
+    if (a.k.type == B200_TYPE_Q4_0 && (a.hd == 64 || a.hd == 128) && !a.kv_index && !a.has_mask && a.softcap == 0.0f && a.Tq * a.gqa <= 8) {
+        const int64_t rb = a.hd / 32 * 18;
+        const auto words = [](const View& x) { return ((uintptr_t)x.p | (uintptr_t)x.nb2 | (uintptr_t)x.nb3) % 4 == 0; };
+        if (a.k.nb1 == rb && a.v.nb1 == rb && words(a.k) && words(a.v)) return kDecRegQ4;
+    }
     return kDecSync;
 }
+
+size_t q4_smem(int hd, int nw) { return (size_t)8 * hd * sizeof(__half) + (size_t)kDecQ4Stages * nw * 2 * (16 * (hd / 32 * 18) + kDecQ4Skew); }
 
 // The keys-on-M kernel: at most 8 query rows, plain form.
 bool q8t_form(const FattnArgs& a) { return !a.has_mask && a.softcap == 0.0f && !a.causal && a.Tq * a.gqa <= 8; }
@@ -2041,8 +2059,31 @@ int launch_decode_q8reg(const FattnArgs& a, cudaStream_t st) {
 }
 
 template <int HD>
+int launch_decode_q4(const FattnArgs& a, cudaStream_t st) {
+    dim3 grid(a.n_splits, a.Hkv, a.B);
+    cudaError_t e;
+    auto go = [&](auto kern, int nw, bool (&smem_set)[64]) {
+        const size_t main = q4_smem(HD, nw), push = use_cluster_merge(a) ? cluster_push_bytes(HD, a.Tq * a.gqa) : 0;
+        e = set_smem_once(kern, main + cluster_push_bytes(HD, 8), smem_set);
+        if (e == cudaSuccess) launch_split(kern, grid, main + push, st, a, 32 * nw);
+    };
+    static bool set[4][64] = {};
+    const bool few = a.Tq * a.gqa <= 4;
+    if (a.wide) few ? go(fattn_decode_q4_kernel<HD, 8, true>, 8, set[0]) : go(fattn_decode_q4_kernel<HD, 8, false>, 8, set[1]);
+    else few ? go(fattn_decode_q4_kernel<HD, 4, true>, 4, set[2]) : go(fattn_decode_q4_kernel<HD, 4, false>, 4, set[3]);
+    if (e != cudaSuccess) return (int)e;
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return (int)e;
+    if (a.n_splits > 1 && !use_cluster_merge(a)) e = launch_merge<HD>(a, st);
+    return (int)e;
+}
+
+template <int HD>
 int launch_decode_t(const FattnArgs& a, cudaStream_t st) {
     switch (decode_mode(a, HD)) {
+        case kDecRegQ4:
+            if constexpr (HD == 64 || HD == 128) return launch_decode_q4<HD>(a, st);
+            else return launch_decode_m<HD, kDecSync>(a, st);
         case kDecRegQ8:
             if constexpr (HD == 64 || HD == 128) return launch_decode_q8reg<HD>(a, st);
             else return launch_decode_m<HD, kDecAsyncQ8>(a, st);
@@ -2238,7 +2279,7 @@ int launch_bounded_wait_probe(int polls, cudaStream_t st) {
 }
 
 bool decode_cluster_merge_ok(const FattnArgs& a) {
-    return cluster_merge_enabled() && (a.k.type == B200_TYPE_Q8_0 || a.k.type == B200_TYPE_F16) && (a.hd == 64 || a.hd == 128);
+    return cluster_merge_enabled() && (is_blocks(a.k.type) || a.k.type == B200_TYPE_F16) && (a.hd == 64 || a.hd == 128);
 }
 
 // CTAs of the split kernel that fit on one SM for these operands (shared memory of the staging form; registers
@@ -2255,6 +2296,11 @@ int decode_ctas_per_sm(const FattnArgs& a, bool cluster) {
             }
             smem = (size_t)kDecRows * hdp * 2 + (size_t)kDecRegStages * 2 * kDecBN * (hdp / 32 * 34);
             break;
+        case kDecRegQ4: {
+            smem = q4_smem(hdp, a.wide ? 8 : 4) + (cluster ? cluster_push_bytes(hdp, a.Tq * a.gqa) : 0);
+            const int n = (int)((size_t)227 * 1024 / (smem + 1536 + 1024)), most = a.wide ? 2 : 4;
+            return n < 1 ? 1 : (n > most ? most : n);
+        }
         case kDecAsyncF16: {
             const int ns = hdp >= 128 ? 3 : 4;
             smem = (size_t)(kDecRows + ns * 2 * kDecBN) * hdp * 2;
@@ -2315,7 +2361,8 @@ int decode_split_choose(FattnArgs& a, int B, int sm_count) {
     // leaves an SM with two CTAs, and a warp's chain through a tile (copy, dequantise, two products) sets the pace.  Eight
     // warps per CTA split the keys once more without a merge outside the CTA: 32 streams x 8 KV heads, 535 keys, 16.5 ->
     // 11.3 us per launch (two splits through the workspace: 13.7).
-    if (best == 1 && units <= 2.0 * sm_count && tiles > 2 && decode_mode(a, a.hd) == kDecRegQ8 && q8t_form(a)) a.wide = 1;
+    const int mode = decode_mode(a, a.hd);
+    if (best == 1 && units <= 2.0 * sm_count && tiles > 2 && ((mode == kDecRegQ8 && q8t_form(a)) || mode == kDecRegQ4)) a.wide = 1;
     return best;
 }
 

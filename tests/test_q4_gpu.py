@@ -350,3 +350,81 @@ def test_tensors_keep_the_cache_alive(b200):
     gc.collect()
     junk = [torch.zeros(1 << 16, device="cuda") for _ in range(8)]
     assert np.array_equal(k.cpu().numpy(), want) and junk
+
+
+# ---- the kernel of the serving form: at most 8 query rows per KV head, head_dim 64 / 128 -----------------------------
+
+# Its result is that of 32-bit arithmetic.  A score is a sum of hd products of exact operands, accumulated in fp32: off by some 2^-22 of
+# the sum of their magnitudes, which for N(0,1) operands is up to 2^3 in log2 units: 2^-19, and so is P.  Weights and the values' sums add
+# 2^-21 each.  An output is a weighted mean in which these errors are independent: relative L2 2^-18 and less.  2^-17 is allowed.
+EXACT_REL = 2.0 ** -17
+
+
+def _exact(got, ref, what):
+    assert np.isfinite(got).all(), what
+    assert errors(got, ref)[1] <= EXACT_REL, f"{what}: {errors(got, ref)}"
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("gqa,Tq", [(1, 1), (3, 1), (4, 1), (1, 5), (8, 1), (2, 3)])
+@pytest.mark.parametrize("B,L", [(1, 97), (3, 700), (40, 333), (2, 9001)])
+def test_serving_form_is_exact(b200, hd, gqa, Tq, B, L):
+    rng = np.random.default_rng(hd + gqa + Tq + L)
+    Hkv = 5
+    k, v, kf, vf = _caches(rng, B, Hkv, L, hd)
+    q = randn_f16(rng, (B, Hkv * gqa, Tq, hd))
+    kw = dict(scale=hd ** -0.5, kv_len=rng.integers(0, L + 1, B).astype(np.int32))
+    kw["kv_len"][0] = L
+    _exact(gpu_op(b200, q, k, v, kv_type=abi.Q4_0, **kw), attention_f64(q, kf, vf, **kw), "plain")
+    if Tq > 1:
+        kw.update(causal=True, q_len=np.minimum(kw["kv_len"], rng.integers(1, Tq + 1, B)).astype(np.int32))
+        _exact(gpu_op(b200, q, k, v, kv_type=abi.Q4_0, **kw), attention_f64(q, kf, vf, **kw), "causal")
+
+
+@pytest.mark.parametrize("case", ["tiny_q", "huge_q", "mixed_q", "tiny_v", "huge_v", "mixed_v", "one_key_wins", "growing_scores", "f32_q", "negative_scale"])
+@pytest.mark.parametrize("gqa", [4, 8])
+def test_serving_form_keeps_its_bits(b200, case, gqa):
+    """Query rows and value blocks of any magnitude, maxima that keep growing, scales that force the weights' range down."""
+    rng = np.random.default_rng(len(case) + gqa)
+    B, Hkv, L, hd, scale = 2, 2, 500, 128, 128 ** -0.5
+    kx, vx = (rng.standard_normal((B, Hkv, L, hd)).astype(np.float32) for _ in "kv")
+    q = rng.standard_normal((B, Hkv * gqa, 1, hd)).astype(np.float32)
+    if case == "tiny_q":
+        q, scale = q * 1e-5, scale * 1e5
+    elif case == "huge_q":
+        q, scale = q * 5000, scale / 5000
+    elif case == "mixed_q":
+        q *= 10.0 ** rng.integers(-4, 1, q.shape)
+    elif case == "tiny_v":
+        vx *= 1e-3
+    elif case == "huge_v":
+        vx *= 9000
+    elif case == "mixed_v":
+        vx[:, :, ::37] *= 400
+    elif case == "one_key_wins":
+        kx[:, 0, 333] = 6 * np.sign(q[:, 0, 0])
+    elif case == "growing_scores":
+        kx = (0.02 * np.arange(L)[:, None] * np.sign(q[:, ::gqa]) * rng.uniform(0.5, 1, kx.shape)).astype(np.float32)
+    elif case == "negative_scale":
+        scale = -scale
+    k, v = quantize_q4_0(kx), quantize_q4_0(vx)
+    kf, vf = dequantize_q4_0(k), dequantize_q4_0(v)
+    q = q if case == "f32_q" else q.astype(np.float16)
+    got = gpu_op(b200, q, k, v, scale=scale, kv_type=abi.Q4_0)
+    ref = attention_f64(q, kf, vf, scale)
+    # scores of 2^8 (growing) or 2^5 (one key) in log2 units: 2^-24 of them more; a Q of 1e-5 has 8 bits below F16's smallest value, all of them kept
+    bound = EXACT_REL * {"growing_scores": 16, "one_key_wins": 4, "mixed_v": 2}.get(case, 1)
+    assert np.isfinite(got).all() and errors(got, ref)[1] <= bound, errors(got, ref)
+
+
+@pytest.mark.parametrize("shift", [0, 4, 8, 12])
+def test_serving_form_on_word_boundaries(b200, shift):
+    """Heads that start anywhere on a 4-byte boundary: rows of 36 bytes, odd row counts, shifted bases of K alone."""
+    rng = np.random.default_rng(shift)
+    for hd, L in ((64, 101), (128, 101), (128, 64)):
+        k, v, kf, vf = _caches(rng, 2, 3, L, hd)
+        base = np.zeros(shift + k.size, np.uint8)
+        base[shift:] = k.reshape(-1)
+        q = randn_f16(rng, (2, 6, 1, hd))
+        got = gpu_op(b200, q, cuda_view(base[shift:].reshape(k.shape), base), v, scale=0.1, kv_type=abi.Q4_0)
+        _exact(got, attention_f64(q, kf, vf, 0.1), f"{hd} {L}")
