@@ -1831,13 +1831,62 @@ __global__ void __launch_bounds__(kThreads) fattn_merge_kernel(const FattnArgs a
     }
 }
 
+// The same with the four warps of a CTA on one row, each on every fourth split: one round of loads for up to 64 splits, where
+// one warp makes a round of memory latency for every sixteen (one stream of 65535 Q4_0 keys, 8 KV heads, 37 splits: 28.2 -> 25.2 us per
+// launch).  For the few rows of such launches; many rows with few splits each keep a warp per row.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) fattn_merge_many_kernel(const FattnArgs a) {
+    constexpr int V = HD / 32;
+    __shared__ float s_o[4][HD], s_m[4], s_l[4];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = a.Tq * a.gqa;
+    const int rr = blockIdx.x % R, hk = (blockIdx.x / R) % a.Hkv, b = blockIdx.x / (R * a.Hkv);
+    const int64_t unit0 = ((int64_t)b * a.Hkv + hk) * a.n_splits;
+    float2 ml[16];
+    float po[16][V], M = -INFINITY, L = 0.0f, acc[V];
+#pragma unroll
+    for (int u = 0; u < 16; u++) {
+        const int s = min(warp + 4 * u, a.n_splits - 1);
+        ml[u] = *reinterpret_cast<const float2*>(a.ws_ml + ((unit0 + s) * kDecRows + rr) * 2);
+        const float* p = a.ws_o + ((unit0 + s) * kDecRows + rr) * HD;
+#pragma unroll
+        for (int i = 0; i < V; i++) po[u][i] = p[lane + 32 * i];
+    }
+#pragma unroll
+    for (int u = 0; u < 16; u++)
+        if (warp + 4 * u < a.n_splits) M = fmaxf(M, ml[u].x);
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[i] = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 16; u++) {
+        if (warp + 4 * u >= a.n_splits || ml[u].x == -INFINITY) continue;
+        const float w = exp2f(ml[u].x - M);
+        L += w * ml[u].y;
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[i] += w * po[u][i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) s_o[warp][lane + 32 * i] = acc[i];
+    if (lane == 0) s_m[warp] = M, s_l[warp] = L;
+    __syncthreads();
+    const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    float w[4], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = s_m[i] == -INFINITY ? 0.0f : exp2f(s_m[i] - top), sum += w[i] * s_l[i];
+    int iq, hq;
+    row_to_query(a, hk, rr, iq, hq);
+    const float inv = (sum > 0.0f && iq < q_rows_of(a, b)) ? 1.0f / sum : 0.0f;
+    float* out = a.dst + (((int64_t)b * a.Tq + iq) * a.dst_heads + hq) * a.hd;
+    for (int c = threadIdx.x; c < a.hd; c += kThreads) out[c] = (w[0] * s_o[0][c] + w[1] * s_o[1][c] + w[2] * s_o[2][c] + w[3] * s_o[3][c]) * inv;
+}
+
 // Merge kernel with programmatic stream serialisation (its launch overlaps the tail of the split kernel; the
 // kernel itself waits for the split grid before it reads the workspace).
 template <int HD>
-cudaError_t launch_merge(const FattnArgs& a, cudaStream_t st) {
+cudaError_t launch_merge(const FattnArgs& a, cudaStream_t st, bool many = false) {
     const int warps = a.B * a.Hkv * a.Tq * a.gqa;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((warps + 3) / 4);
+    cfg.gridDim = dim3(many ? warps : (warps + 3) / 4);
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = 0;
     cfg.stream = st;
@@ -1846,7 +1895,7 @@ cudaError_t launch_merge(const FattnArgs& a, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fattn_merge_kernel<HD>, a);
+    return many ? cudaLaunchKernelEx(&cfg, fattn_merge_many_kernel<HD>, a) : cudaLaunchKernelEx(&cfg, fattn_merge_kernel<HD>, a);
 }
 
 // The splits of one (batch entry, kv-head) of the Q8_0 register kernel run as one thread-block cluster when there
@@ -1864,12 +1913,16 @@ bool cluster_merge_enabled() {
     return enabled;
 }
 
+// Clusters of the Q4_0 kernel find no place on the last SMs of a nearly full grid: 4 streams x 20 KV heads, 1500 keys, 480 CTAs in clusters of
+// six 6.9 us, 560 in clusters of seven 10.4.
+constexpr double kQ4ClusterFill = 0.87;
+
 bool use_cluster_merge(const FattnArgs& a) {
     // only while the whole grid is resident at once (2 to 4 CTAs on each of 148 SMs): with several waves the cluster
     // barriers hold finished CTAs on their SMs and the form measured 10 % slower than the merge kernel.  Pairs at head_dim 64 over an F16
     // cache hold little and save the merge kernel (32 segments of the large decoder 101.6 -> 97.5 us per layer).
     return decode_cluster_merge_ok(a) && a.n_splits > 1 && a.n_splits <= 8 && ((a.n_splits == 2 && a.k.type == B200_TYPE_F16 && a.hd == 64) ||
-           (long)a.n_splits * a.Hkv * a.B <= (long)decode_ctas_per_sm(a, true) * 148);
+           (long)a.n_splits * a.Hkv * a.B <= (long)decode_ctas_per_sm(a, true) * 148 * (a.k.type == B200_TYPE_Q4_0 ? kQ4ClusterFill : 1.0));
 }
 
 template <typename Kern>
@@ -2011,7 +2064,7 @@ int decode_mode(const FattnArgs& a, int hdp) {
     return kDecSync;
 }
 
-size_t q4_smem(int hd, int nw) { return (size_t)8 * hd * sizeof(__half) + (size_t)kDecQ4Stages * nw * 2 * (16 * (hd / 32 * 18) + kDecQ4Skew); }
+size_t q4_smem(int hd, int nw) { return (size_t)8 * hd * sizeof(__half) + (size_t)kDecQ4Stages * nw * 2 * (kDecQ4Keys * (hd / 32 * 18) + kDecQ4Skew); }
 
 // The keys-on-M kernel: at most 8 query rows, plain form.
 bool q8t_form(const FattnArgs& a) { return !a.has_mask && a.softcap == 0.0f && !a.causal && a.Tq * a.gqa <= 8; }
@@ -2074,7 +2127,7 @@ int launch_decode_q4(const FattnArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return (int)e;
     e = cudaGetLastError();
     if (e != cudaSuccess) return (int)e;
-    if (a.n_splits > 1 && !use_cluster_merge(a)) e = launch_merge<HD>(a, st);
+    if (a.n_splits > 1 && !use_cluster_merge(a)) e = launch_merge<HD>(a, st, a.n_splits > 8);
     return (int)e;
 }
 
@@ -2324,6 +2377,43 @@ int decode_ctas_per_sm(const FattnArgs& a, bool cluster) {
 static std::atomic<int> g_forced_splits{0};
 void decode_split_force(int n_splits) { g_forced_splits.store(n_splits, std::memory_order_relaxed); }
 
+// Split count and warps per CTA over a Q4_0 cache, whose kernel is bound by its instructions and not by the bytes that a CTA has in
+// flight: what counts is how many warps an SM's schedulers have and how evenly the SMs are filled.  In units of one
+// 32-key step of a CTA that has its SM to itself (1.03 us at head_dim 128): a step of two, three or four warps per scheduler takes
+// 1.5, 2.0 and 2.45; launches that do not fit take as many passes over the SMs, each with its set-up; splits of a resident grid
+// merge inside clusters, others through the workspace.  Fitted to 28 launches of 1 to 256 streams, 97 to 65535 keys, 2 to 20 KV heads at head_dim
+// 64 and 128, all split counts with four and with eight warps per CTA: what it picks is within 1 % of the best but for 512
+// units (78.8 us against 75.5 in two splits).  Eight warps: 8 streams x 2000 keys 10.6 -> 10.0 us, one of 4000 7.9 -> 6.6, 16 of 535 9.1 -> 6.8.
+int q4_choose(FattnArgs& a, int B, int sm_count) {
+    const int Lk = a.Lk;
+    const double units = (double)B * a.Hkv, f = a.hd == 128 ? 1.0 : 0.55;
+    constexpr double kStep[5] = {0.0, 1.0, 1.5, 2.0, 2.45};
+    int best = 1;
+    double best_cost = 0.0;
+    for (int wide = 0; wide < 2; wide++) {
+        const int nw = wide ? 8 : 4, keys = kDecQ4Keys * nw, tiles = (Lk + keys - 1) / keys, resident = 16 / nw;
+        a.wide = wide;
+        const bool cluster_ok = decode_cluster_merge_ok(a);
+        for (int n = 1; n <= tiles && n <= 64; n++) {
+            const int tps = (tiles + n - 1) / n;
+            if ((tiles + tps - 1) / tps != n) continue;   // some split would get no tile
+            const double share = fmax((double)Lk / keys / n, tps - 1.0), steps = 0.35 * tps + 0.65 * fmin(share, (double)tps);   // the last tile's missing keys
+            const double ctas = units * n, per_sm = ceil(ctas / sm_count);
+            double cost;
+            if (per_sm <= resident) {
+                cost = steps * f * kStep[(int)per_sm * nw / 4] + 0.3 * (per_sm - 1.0) * nw / 4;
+            } else {
+                const double x = ctas / (sm_count * resident), passes = x <= 2.0 ? ceil(x) : x + 0.2;
+                cost = passes * (steps * f * kStep[4] + 2.5 + wide);
+            }
+            if (n > 1) cost += cluster_ok && n <= 8 && ctas <= kQ4ClusterFill * sm_count * resident ? 0.8 + 0.03 * n : 2.4 + 0.08 * n;
+            if ((wide == 0 && n == 1) || cost < best_cost - 1e-9) best = n | wide << 8, best_cost = cost;
+        }
+    }
+    a.wide = best >> 8;
+    return best & 255;
+}
+
 int decode_split_choose(FattnArgs& a, int B, int sm_count) {
     a.wide = 0;
     const int forced = g_forced_splits.load(std::memory_order_relaxed);
@@ -2335,6 +2425,7 @@ int decode_split_choose(FattnArgs& a, int B, int sm_count) {
     const int tiles = ((a.kv_index ? a.kv_index_stride : a.Lk) + kDecBN - 1) / kDecBN;
     if (tiles <= 1) return 1;
     if (forced) return forced < tiles ? forced : tiles;
+    if (decode_mode(a, a.hd) == kDecRegQ4) return q4_choose(a, B, sm_count);
     const double units = (double)B * a.Hkv;
     const double cap = (double)(per_sm_env ? per_sm_env : decode_ctas_per_sm(a)) * sm_count;
     const double cap_cluster = (double)(per_sm_env ? per_sm_env : decode_ctas_per_sm(a, true)) * sm_count;   // with the receive area of the merge
@@ -2361,8 +2452,7 @@ int decode_split_choose(FattnArgs& a, int B, int sm_count) {
     // leaves an SM with two CTAs, and a warp's chain through a tile (copy, dequantise, two products) sets the pace.  Eight
     // warps per CTA split the keys once more without a merge outside the CTA: 32 streams x 8 KV heads, 535 keys, 16.5 ->
     // 11.3 us per launch (two splits through the workspace: 13.7).
-    const int mode = decode_mode(a, a.hd);
-    if (best == 1 && units <= 2.0 * sm_count && tiles > 2 && ((mode == kDecRegQ8 && q8t_form(a)) || mode == kDecRegQ4)) a.wide = 1;
+    if (best == 1 && units <= 2.0 * sm_count && tiles > 2 && decode_mode(a, a.hd) == kDecRegQ8 && q8t_form(a)) a.wide = 1;
     return best;
 }
 
