@@ -16,6 +16,7 @@
 #include <atomic>
 #include <cstdlib>
 #include "fattn_common.cuh"
+#include "kv_rows.cuh"
 
 namespace b200 {
 
@@ -2212,6 +2213,14 @@ __global__ void __launch_bounds__(256) kv_to_f16_kernel(const View src0, uint8_t
                 }
                 out[(int64_t)(row0 + u * RPW) * LPR] = make_uint4(o[0], o[1], o[2], o[3]);
             }
+    } else if constexpr (TYPE == B200_TYPE_Q4_0 && VEC16) {   // the same: 8 streams x 407 rows x 8 heads CAST_OLD -> CAST_NEW us
+        Row8<TYPE, true> x[kCastUnroll];
+#pragma unroll
+        for (int u = 0; u < kCastUnroll; u++)
+            if (row0 + u * RPW < Lk) x[u].load(base + (int64_t)(row0 + u * RPW) * src.nb1, c);
+#pragma unroll
+        for (int u = 0; u < kCastUnroll; u++)
+            if (row0 + u * RPW < Lk) out[(int64_t)(row0 + u * RPW) * LPR] = x[u].halves(c);
     } else {   // unaligned rows
 #pragma unroll
         for (int u = 0; u < kCastUnroll; u++)
@@ -2244,7 +2253,8 @@ int launch_cast_any(const View& k, void* kdst, const View& v, void* vdst, int n,
                                                             : launch_cast<B200_TYPE_F32, false>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st));
         case B200_TYPE_Q8_0: return (int)(words(k) && words(v) ? launch_cast<B200_TYPE_Q8_0, true>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st)
                                                                : launch_cast<B200_TYPE_Q8_0, false>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st));
-        case B200_TYPE_Q4_0: return (int)launch_cast<B200_TYPE_Q4_0, false>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st);
+        case B200_TYPE_Q4_0: return (int)(words(k) && words(v) ? launch_cast<B200_TYPE_Q4_0, true>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st)
+                                                               : launch_cast<B200_TYPE_Q4_0, false>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st));
         default: return (int)(k.vec16 && v.vec16 ? launch_cast<B200_TYPE_F16, true>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st)
                                                  : launch_cast<B200_TYPE_F16, false>(k, kdst, v, vdst, n, hd, Lk, Hkv, Bk, st));
     }

@@ -57,7 +57,7 @@ __device__ __forceinline__ void store_row8(uint8_t* row_out, int c, const float 
         const int blk = c >> 5, i4 = (c & 31) >> 3;   // lane i4 of the block's four
         if constexpr (TYPE == B200_TYPE_Q8_0) {
             const float d = __fdiv_rn(amax, 127.0f);
-            const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+            const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
             uint32_t q[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) q[i] = round_away(__fmul_rn(f[i], id));
@@ -92,7 +92,7 @@ __device__ __forceinline__ void store_row8(uint8_t* row_out, int c, const float 
             const uint32_t has = __ballot_sync(0xffffffffu, own == amax) >> (threadIdx.x & 28) & 15u;
             sign = __shfl_sync(0xffffffffu, sign, has ? __ffs(has) - 1 : 0, 4);
             const float d = amax * (sign ? 0.125f : -0.125f);   // (a power of two: exact but for denormals, where d is 0 in fp16)
-            const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+            const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
             uint32_t w0 = 0, w1 = 0;
 #pragma unroll
             for (int i = 3; i >= 0; i--) {
@@ -115,34 +115,127 @@ __device__ __forceinline__ void store_row8(uint8_t* row_out, int c, const float 
     }
 }
 
-// Eight values [c, c + 8) of the cache row at `row`, which a kernel before this one may have written.
+// The same for lanes that hold four values of each half of a row, f[0..3] = [4 l, 4 l + 4) and f[4..7] = hd/2 + [4 l, 4 l + 4): eight lanes
+// (from a multiple of eight) share a block of either half.  hd is 64 or 128, l the lane's place in its row.
 template <int TYPE>
-__device__ __forceinline__ void load_row8(const uint8_t* row, int c, float (&f)[8]) {
-    if constexpr (TYPE == B200_TYPE_F16) {
-        const uint4 u = load_global(reinterpret_cast<const uint4*>(row + 2 * c));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+__device__ __forceinline__ void store_row4x2(uint8_t* row_out, int l, const float (&f)[8], bool live, int hd) {
+    const int i8 = l & 7;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            f[2 * i] = p.x, f[2 * i + 1] = p.y;
+    for (int part = 0; part < 2; part++) {
+        const float* x = f + 4 * part;
+        if constexpr (TYPE == B200_TYPE_F16) {
+            if (live) *reinterpret_cast<uint2*>(row_out + part * hd + 8 * l) = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+            continue;
         }
-    } else {
-        constexpr int BB = TYPE == B200_TYPE_Q8_0 ? 34 : 18;
-        const uint8_t* blk = row + BB * (c >> 5);
-        const float d = __half2float(__ushort_as_half(load_global(reinterpret_cast<const uint16_t*>(blk))));
-        const uint16_t* qs = reinterpret_cast<const uint16_t*>(blk + 2 + (TYPE == B200_TYPE_Q8_0 ? c & 31 : c & 15));
-        const int sh = (c & 16) ? 4 : 0;
+        const int blk = (l >> 3) + part * (hd / 64);
+        const float own = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+        float amax = own;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t w = load_global(qs + i);
-            if (TYPE == B200_TYPE_Q8_0) {
-                f[2 * i] = d * (float)(int8_t)(w & 0xFF), f[2 * i + 1] = d * (float)(int8_t)(w >> 8);
-            } else {
-                f[2 * i] = d * (float)((int)(w >> sh & 15u) - 8), f[2 * i + 1] = d * (float)((int)(w >> (8 + sh) & 15u) - 8);
+        for (int m = 1; m < 8; m <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
+        if constexpr (TYPE == B200_TYPE_Q8_0) {
+            const float d = __fdiv_rn(amax, 127.0f);
+            const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
+            const uint32_t w = low_bytes(round_away(__fmul_rn(x[0], id)), round_away(__fmul_rn(x[1], id)), round_away(__fmul_rn(x[2], id)), round_away(__fmul_rn(x[3], id)));
+            const uint32_t dbits = __half_as_ushort(__float2half_rn(d)), left = __shfl_up_sync(0xffffffffu, w, 1);
+            if (!live) continue;
+            uint8_t* out = row_out + blk * 34 + 4 * i8;
+            if (blk & 1) {
+                *reinterpret_cast<uint32_t*>(out + 2) = w;
+                if (i8 == 0) *reinterpret_cast<uint16_t*>(out) = (uint16_t)dbits;
+            } else {   // (the block's quants are two bytes off the words' boundaries)
+                *reinterpret_cast<uint32_t*>(out) = (w << 16) | (i8 == 0 ? dbits : left >> 16);
+                if (i8 == 7) *reinterpret_cast<uint16_t*>(out + 4) = (uint16_t)(w >> 16);
             }
+        } else if constexpr (TYPE == B200_TYPE_Q4_0) {
+            uint32_t sign = 0;
+#pragma unroll
+            for (int i = 3; i >= 0; i--)
+                if (fabsf(x[i]) == amax) sign = __float_as_uint(x[i]) >> 31;
+            const uint32_t has = __ballot_sync(0xffffffffu, own == amax) >> (threadIdx.x & 24) & 255u;
+            sign = __shfl_sync(0xffffffffu, sign, has ? __ffs(has) - 1 : 0, 8);
+            const float d = amax * (sign ? 0.125f : -0.125f);
+            const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 3; i >= 0; i--) w = (w << 8) | (nibble_of(x[i], id) & 15u);
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, w, 4);   // values 16.. of the block are lanes 4..7's
+            w = i8 < 4 ? w | (other << 4) : other | (w << 4);
+            if (!live) continue;
+            uint8_t* out = row_out + blk * 18;
+            *reinterpret_cast<uint16_t*>(out + 2 + 4 * (i8 & 3) + (i8 < 4 ? 0 : 2)) = (uint16_t)(i8 < 4 ? w : w >> 16);
+            if (i8 == 0) *reinterpret_cast<uint16_t*>(out) = __half_as_ushort(__float2half_rn(d));
         }
     }
 }
+
+// Eight values [c, c + 8) of a row of blocks as they lie in memory, loaded and then converted, so that the loads of several rows can be in flight.  The
+// kernel before this one may have written the row.  WORDS: rows on 4-byte boundaries.  The eight quants start 2 + 8 i bytes into
+// their block, in odd blocks (34 and 18 bytes) on a word's boundary, in even ones two bytes off one, where a third word makes them up.
+template <int TYPE, bool WORDS, bool SHARED = false>
+struct Row8 {
+    uint32_t w[TYPE == B200_TYPE_F16 ? 4 : 2];
+    uint16_t d;
+
+    // (from global memory behind griddepcontrol.wait, or from shared memory)
+    template <typename T>
+    static __device__ __forceinline__ T get(const T* p) {
+        if constexpr (SHARED) return *p;
+        else return load_global(p);
+    }
+    __device__ __forceinline__ void load(const uint8_t* row, int c) {
+        if constexpr (TYPE == B200_TYPE_F16) {
+            const uint4 u = get(reinterpret_cast<const uint4*>(row + 2 * c));
+            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        } else {
+            const int blk = c >> 5, odd = blk & 1, first = TYPE == B200_TYPE_Q8_0 ? c & 31 : c & 15;
+            const uint8_t* p = row + (TYPE == B200_TYPE_Q8_0 ? 34 : 18) * blk;
+            if constexpr (WORDS) {
+                const uint32_t* x = reinterpret_cast<const uint32_t*>(p + first + 2 * odd);
+                w[0] = get(x), w[1] = get(x + 1);
+                if (!odd) {
+                    const uint32_t last = get(reinterpret_cast<const uint16_t*>(x + 2));
+                    w[0] = __funnelshift_r(w[0], w[1], 16), w[1] = __byte_perm(w[1], last, 0x5432);
+                }
+            } else {
+                const uint16_t* x = reinterpret_cast<const uint16_t*>(p + 2 + first);
+                w[0] = get(x) | (uint32_t)get(x + 1) << 16, w[1] = get(x + 2) | (uint32_t)get(x + 3) << 16;
+            }
+            d = get(reinterpret_cast<const uint16_t*>(p));
+        }
+    }
+    __device__ __forceinline__ void values(int c, float (&f)[8]) const {
+        if constexpr (TYPE == B200_TYPE_F16) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                f[2 * i] = p.x, f[2 * i + 1] = p.y;
+            }
+        } else {
+            const float scale = __half2float(__ushort_as_half(d));
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t x = w[i >> 2] >> (8 * (i & 3));
+                f[i] = scale * (float)(TYPE == B200_TYPE_Q8_0 ? (int)(int8_t)x : (int)(x >> (c & 16 ? 4 : 0) & 15u) - 8);
+            }
+        }
+    }
+    // The same rounded to F16 (blocks only): the quants as exact halves, one product, one rounding.
+    __device__ __forceinline__ uint4 halves(int c) const {
+        uint32_t o[4];
+        const __half2 d2 = __half2half2(__ushort_as_half(d));
+        // halves 0x64xx = 1024 + xx, less 1152 (int8 with its sign bit flipped) or 1032 (nibbles)
+        const __half2 bias = __float2half2_rn(TYPE == B200_TYPE_Q8_0 ? 1152.0f : 1032.0f);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const uint32_t q = TYPE == B200_TYPE_Q8_0 ? w[k] ^ 0x80808080u : (c & 16 ? w[k] >> 4 : w[k]) & 0x0F0F0F0Fu;
+            const uint32_t h01 = __byte_perm(q, 0x64646464u, 0x4140), h23 = __byte_perm(q, 0x64646464u, 0x4342);
+            const __half2 v01 = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&h01), bias), d2);
+            const __half2 v23 = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&h23), bias), d2);
+            o[2 * k] = *reinterpret_cast<const uint32_t*>(&v01), o[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&v23);
+        }
+        return make_uint4(o[0], o[1], o[2], o[3]);
+    }
+};
 
 // Eight consecutive values out, rounded to F16 or as they are; V16: 16-byte aligned addresses.
 template <bool F32, bool V16>

@@ -7,6 +7,7 @@
 // 16-byte boundary for all row sizes (a Q8_0 row of head_dim 128 is 136 bytes, a Q4_0 row 72).
 #include <cstdio>
 #include <new>
+#include <type_traits>
 
 #include "kv_cache.h"
 #include "kv_rows.cuh"
@@ -127,40 +128,70 @@ struct ReadArgs {
     const int32_t* pos;
 };
 
-template <int TYPE, bool F32, bool V16>
-__global__ void __launch_bounds__(256) kv_read_kernel(const ReadArgs a) {
+// Bound by its bytes.  The rows of a head are one range of bytes, of which a CTA brings kReadRows rows into shared memory by 16-byte copies
+// (from the unit around the first row on: rows start on 2-, 4- or 8-byte boundaries) and takes them apart there: with loads of words
+// and halves straight from the cache, four rows in flight per lane, the lanes waited for them most of the time (8 x 1500 rows of 8 heads, Q8_0:
+// READ_OLD us, this form READ_NEW).
+constexpr int kReadRows = 64, kReadThreads = 128;
+
+template <int TYPE, bool F32, bool V16, bool WORDS>
+__global__ void __launch_bounds__(kReadThreads) kv_read_kernel(const ReadArgs a) {
     let_dependents_launch();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int lpr = a.hd / 8, rpw = 32 / lpr, sub = lane / lpr, c = (lane - sub * lpr) * 8;
-    const int which = blockIdx.y, sh = blockIdx.x / a.chunks, chunk = blockIdx.x - sh * a.chunks, s = sh / a.n_kv, h = sh - s * a.n_kv;
+    extern __shared__ __align__(16) uint8_t s_rows[];
+    const int which = blockIdx.y, sh = blockIdx.x / a.chunks, row0 = (blockIdx.x - sh * a.chunks) * kReadRows, s = sh / a.n_kv, h = sh - s * a.n_kv;
+    const int rows = min(kReadRows, a.n - row0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (sub >= rpw) return;
-    const int64_t p0 = a.pos ? a.pos[s] : a.pos0;
-    const uint8_t* src = a.src[which] + (int64_t)h * a.snb2 + (int64_t)s * a.snb3;
+    const int64_t first = (int64_t)(a.pos ? a.pos[s] : a.pos0) + row0;   // cache row of the CTA's first row
+    const int lo = (int)min((int64_t)rows, max((int64_t)0, -first)), hi = (int)max((int64_t)lo, min((int64_t)rows, a.ctx_rows - first));   // rows [lo, hi) are there
+    const uint8_t* src = a.src[which] + (int64_t)h * a.snb2 + (int64_t)s * a.snb3 + (first + lo) * a.snb1;
+    const int skew = (int)((uintptr_t)src & 15), units = hi > lo ? (int)((skew + (hi - lo) * a.snb1 + 15) / 16) : 0;
+    for (int i = threadIdx.x; i < units; i += kReadThreads)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(s_rows + 16 * i)), "l"(src - skew + 16 * i) : "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    const int lpr = a.hd / 8, rpi = kReadThreads / lpr, sub = threadIdx.x / lpr, c = (threadIdx.x - sub * lpr) * 8;   // lanes per row, rows per step
+    if (sub >= rpi) return;
     uint8_t* dst = a.dst[which] + (int64_t)h * a.dnb2[which] + (int64_t)s * a.dnb3[which] + (int64_t)c * (F32 ? 4 : 2);
-    for (int row = (chunk * (blockDim.x >> 5) + warp) * rpw + sub; row < a.n; row += a.chunks * (blockDim.x >> 5) * rpw) {
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (p0 + row >= 0 && p0 + row < a.ctx_rows) load_row8<TYPE>(src + (p0 + row) * a.snb1, c, f);
-        store8<F32, V16>(dst + (int64_t)row * a.dnb1[which], f);
+    for (int row = sub; row < rows; row += rpi) {
+        uint8_t* out = dst + (int64_t)(row0 + row) * a.dnb1[which];
+        const bool there = row >= lo && row < hi;
+        Row8<TYPE, WORDS, true> x;
+        if (there) x.load(s_rows + skew + (row - lo) * (int)a.snb1, c);
+        if constexpr (!F32 && V16) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (TYPE == B200_TYPE_F16) {
+                if (there) v = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
+            } else {
+                if (there) v = x.halves(c);
+            }
+            *reinterpret_cast<uint4*>(out) = v;
+        } else {
+            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (there) x.values(c, f);
+            store8<F32, V16>(out, f);
+        }
     }
 }
 
 template <int TYPE>
 cudaError_t launch_read(ReadArgs a, int n_heads_total, bool f32, bool v16, cudaStream_t st) {
-    const int rpw = 32 / (a.hd / 8), units = (a.n + rpw - 1) / rpw, per_block = units < 8 ? units : 8;
-    const int full = (units + per_block - 1) / per_block, resident = (148 * 8 + 2 * n_heads_total - 1) / (2 * n_heads_total);
-    a.chunks = full < resident ? full : resident;
+    a.chunks = (a.n + kReadRows - 1) / kReadRows;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.chunks * n_heads_total, 2);
-    cfg.blockDim = dim3(32 * per_block);
+    cfg.blockDim = dim3(kReadThreads);
+    cfg.dynamicSmemBytes = (size_t)(a.n < kReadRows ? a.n : kReadRows) * a.snb1 + 32;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (f32) return v16 ? cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, true, true>, a) : cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, true, false>, a);
-    return v16 ? cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, false, true>, a) : cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, false, false>, a);
+    auto go = [&](auto words) {
+        constexpr bool W = decltype(words)::value;
+        if (f32) return v16 ? cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, true, true, W>, a) : cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, true, false, W>, a);
+        return v16 ? cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, false, true, W>, a) : cudaLaunchKernelEx(&cfg, kv_read_kernel<TYPE, false, false, W>, a);
+    };
+    return a.hd % 64 == 0 ? go(std::true_type()) : go(std::false_type());   // an odd number of blocks: rows on 2-byte boundaries
 }
 
 }  // namespace

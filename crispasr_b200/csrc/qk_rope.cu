@@ -7,6 +7,7 @@
 // where many rows enter and by the launch where one does.
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "kv_cache.h"
 #include "kv_rows.cuh"
@@ -26,7 +27,7 @@ struct RopeArgs {
     const float* w[2];       // norm weights of q and k; null = no norm
     int n, hd, n_dims, neox, out_f32, ctx_rows, pos0, chunks;   // chunks: warps per token
     int n_tokens;            // streams x rows
-    float eps;
+    float eps, inv_hd;
     const int32_t* pos;
     const int32_t* n_rows;
     uint64_t turns[kMaxHalf];   // turns per position of each pair, as a fraction of 2^64
@@ -65,17 +66,53 @@ __device__ __forceinline__ void load_in8(const uint8_t* p, float (&f)[8]) {
     }
 }
 
+// Four values of either half of a row (16-byte aligned rows).
+template <bool F32>
+__device__ __forceinline__ void load_in4x2(const uint8_t* p, const uint8_t* q, float (&f)[8]) {
+    if constexpr (F32) {
+        const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(q));
+        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    } else {
+        const uint2 a = __ldcs(reinterpret_cast<const uint2*>(p)), b = __ldcs(reinterpret_cast<const uint2*>(q));
+        const uint32_t u[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+            f[2 * i] = x.x, f[2 * i + 1] = x.y;
+        }
+    }
+}
+__device__ __forceinline__ void store_out4x2(uint8_t* row, int c, const float (&f)[8], int hd, int f32) {
+#pragma unroll
+    for (int part = 0; part < 2; part++) {
+        const float* x = f + 4 * part;
+        const int e = c + part * (hd / 2);
+        if (f32) *reinterpret_cast<float4*>(row + 4 * e) = make_float4(x[0], x[1], x[2], x[3]);
+        else *reinterpret_cast<uint2*>(row + 2 * e) = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+    }
+}
+template <bool V16>
+__device__ __forceinline__ void store_out8(uint8_t* p, const float (&f)[8], int f32) {
+    if (f32) store8<true, V16>(p, f);
+    else store8<false, V16>(p, f);
+}
+
 // A warp takes one token and a run of its rows (the heads of q, then those of k, then of v), eight values per lane, 32 / LPR rows at
-// a time: the cosines and sines of the token's position are worked out once for all of them.
+// a time, the loads of U such groups in flight: the cosines and sines of the token's position are worked out once for all of them, the norm's
+// weights once per tensor.
 // LPR: lanes per row, hd / 8 rounded up to a power of two.  CACHE: type of the cache, or F32 for outputs that are tensors.
-template <bool F32, bool V16, int LPR, int CACHE>
+// HALVES (NEOX, all of a head of 64 or 128 rotated, 16-byte rows): a lane has four values of either half of its row, which are each
+// other's partners: no exchange between lanes, half as many cosines, and 256 contiguous bytes per load of a row.  Otherwise a lane has eight
+// consecutive values, and with NEOX fetches the partners from another lane.
+template <bool F32, bool V16, int LPR, int CACHE, bool HALVES>
 __global__ void __launch_bounds__(32 * kRopeWarps) qk_rope_kernel(const __grid_constant__ RopeArgs a) {
     let_dependents_launch();
     __shared__ uint64_t s_turns[kMaxHalf];
     if (threadIdx.x < a.n_dims / 2) s_turns[threadIdx.x] = a.turns[threadIdx.x];
     __syncthreads();
-    constexpr int RPW = 32 / LPR;
-    const int lane = threadIdx.x & 31, sub = lane / LPR, c = (lane % LPR) * 8, half = a.n_dims / 2;
+    constexpr int RPW = 32 / LPR, ES = F32 ? 4 : 2, U = is_blocks(CACHE) ? 2 : 4;   // groups in flight: block arithmetic wants the registers of two
+    const int lane = threadIdx.x & 31, sub = lane / LPR, l = lane % LPR, half = a.n_dims / 2;
+    const int c = HALVES ? 4 * l : 8 * l;   // the lane's first value
     const int64_t unit = (int64_t)blockIdx.x * kRopeWarps + (threadIdx.x >> 5);
     const int token = (int)(unit / a.chunks), chunk = (int)(unit - (int64_t)token * a.chunks);
     // launched with programmatic stream serialisation: nothing is read before the kernels ahead of this one have completed
@@ -84,59 +121,126 @@ __global__ void __launch_bounds__(32 * kRopeWarps) qk_rope_kernel(const __grid_c
     const int s = token / a.n, i = token - s * a.n;
     const int64_t p = (int64_t)(a.pos ? a.pos[s] : a.pos0) + i;
     const bool valid = !a.n_rows || i < a.n_rows[s];
-    const bool stored = CACHE == B200_TYPE_F32 || (valid && p >= 0 && p < a.ctx_rows);
+    const bool stored = p >= 0 && p < a.ctx_rows;
 
     int groups[3], total = 0;
 #pragma unroll
     for (int x = 0; x < 3; x++) groups[x] = (a.heads[x] + RPW - 1) / RPW, total += groups[x];
     const int per = (total + a.chunks - 1) / a.chunks, lo = chunk * per, hi = min(total, lo + per);
+    const bool inside = c < a.hd;   // (a head of 96 or 80 leaves some of the sixteen lanes without values)
 
-    // value j of the lane: y * cs[j] + partner * sn[j]
-    float cs[8], sn[8];
-    const bool turned = valid && lo < groups[0] + groups[1];
+    if (!valid) {   // a row behind n_rows: zeros to the tensors, nothing to the cache
+        const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        cs[j] = 1.0f, sn[j] = 0.0f;
-        const int e = c + j, pair = a.neox ? (e < half ? e : e - half) : e >> 1;
-        if (turned && e < a.n_dims) {
-            angle_of(s_turns[pair], p, cs[j], sn[j]);
-            if (a.neox ? e < half : !(e & 1)) sn[j] = -sn[j];
-        }
-    }
-    const int partner = a.neox ? (c < half ? lane + half / 8 : lane - half / 8) & 31 : lane;
-
-    for (int grp = lo; grp < hi; grp++) {
-        const int kind = grp < groups[0] ? 0 : (grp < groups[0] + groups[1] ? 1 : 2);
-        const int h = (grp - (kind > 0 ? groups[0] : 0) - (kind > 1 ? groups[1] : 0)) * RPW + sub;
-        const bool live = h < a.heads[kind] && c < a.hd;
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live && valid) load_in8<F32, V16>(a.src[kind] + (int64_t)i * a.snb1[kind] + (int64_t)h * a.snb2[kind] + (int64_t)s * a.snb3[kind] + c * (F32 ? 4 : 2), f);
-        if (kind < 2 && valid) {   // (a row behind n_rows stays zero)
-            if (a.w[kind]) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; j++) sum = fmaf(f[j], f[j], sum);
-#pragma unroll
-                for (int m = LPR / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-                const float r = rsqrtf(sum / (float)a.hd + a.eps);
-#pragma unroll
-                for (int j = 0; j < 8; j++) f[j] = f[j] * r * (c < a.hd ? load_global(a.w[kind] + c + j) : 0.0f);
+        for (int kind = 0; kind < (CACHE == B200_TYPE_F32 ? 2 : 1); kind++)
+            for (int h = sub + chunk * RPW; h < a.heads[kind]; h += a.chunks * RPW) {
+                uint8_t* out = a.dst[kind] + (int64_t)i * a.dnb1[kind] + (int64_t)h * a.dnb2[kind] + (int64_t)s * a.dnb3[kind];
+                if (8 * l < a.hd) store_out8<V16>(out + 8 * l * (a.out_f32 ? 4 : 2), zero, a.out_f32);
             }
-            float other[8];
+        return;
+    }
+
+    // HALVES: pair j of the lane turns by (cs[j], sn[j]); else value j is y * cs[j] + partner * sn[j]
+    float cs[8], sn[8];
+    if (lo < groups[0] + groups[1]) {
+        if constexpr (HALVES) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) other[j] = a.neox ? __shfl_sync(0xffffffffu, f[j], partner) : f[j ^ 1];
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (c + j < a.n_dims) f[j] = fmaf(f[j], cs[j], other[j] * sn[j]);
-        }
-        if (CACHE == B200_TYPE_F32 || kind == 0) {
-            uint8_t* out = a.dst[kind] + (int64_t)i * a.dnb1[kind] + (int64_t)h * a.dnb2[kind] + (int64_t)s * a.dnb3[kind] + c * (a.out_f32 ? 4 : 2);
-            if (live && a.out_f32) store8<true, V16>(out, f);
-            else if (live) store8<false, V16>(out, f);
+            for (int j = 0; j < 4; j++) angle_of(s_turns[c + j], p, cs[j], sn[j]);
         } else {
-            store_row8<CACHE>(a.dst[kind] + (int64_t)h * a.dnb2[kind] + (int64_t)s * a.dnb3[kind] + p * a.dnb1[kind], c, f, live && stored, a.hd);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int e = c + j;
+                cs[j] = 1.0f, sn[j] = 0.0f;
+                if (e >= a.n_dims) continue;
+                if (a.neox || !(j & 1)) angle_of(s_turns[a.neox ? (e < half ? e : e - half) : e >> 1], p, cs[j], sn[j]);
+                else cs[j] = cs[j - 1], sn[j] = -sn[j - 1];   // (the pair's first value has -sin)
+                if (a.neox ? e < half : !(j & 1)) sn[j] = -sn[j];
+            }
         }
     }
+    const int partner = !HALVES && a.neox ? (c < half ? lane + half / 8 : lane - half / 8) & 31 : lane;
+
+    int first = 0;
+    auto rows = [&](auto kind_) {
+        constexpr int kind = decltype(kind_)::value;
+        constexpr bool kTurn = kind < 2, kApart = HALVES && kTurn;   // (v's rows are not rotated: eight consecutive values per lane, one block's arithmetic instead of two)
+        constexpr bool kTensor = CACHE == B200_TYPE_F32 || kind == 0;
+        const int g_lo = max(lo, first) - first, g_hi = min(hi, first + groups[kind]) - first;
+        first += groups[kind];
+        if (g_lo >= g_hi) return;
+        const bool normed = kTurn && a.w[kTurn ? kind : 0] != nullptr;
+        float w[8];
+        if (normed) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = inside ? load_global(a.w[kTurn ? kind : 0] + (HALVES && j >= 4 ? a.hd / 2 - 4 : 0) + c + j) : 0.0f;
+        }
+        const int at = kApart ? c : 8 * l, last = a.heads[kind] - 1;
+        const uint8_t* src = a.src[kind] + (int64_t)i * a.snb1[kind] + (int64_t)s * a.snb3[kind] + (inside ? at : 0) * ES;
+        uint8_t* dst = a.dst[kind] + (int64_t)s * a.dnb3[kind] + (kTensor ? (int64_t)i : p) * a.dnb1[kind];
+        const int64_t src_step = a.snb2[kind], dst_step = a.dnb2[kind];
+        for (int g0 = g_lo; g0 < g_hi; g0 += U) {
+            float f[U][8];
+#pragma unroll
+            for (int u = 0; u < U; u++) {   // lanes behind the last head take its row once more and store nothing
+                const uint8_t* row = src + min((g0 + u) * RPW + sub, last) * src_step;
+                if constexpr (kApart) load_in4x2<F32>(row, row + a.hd / 2 * ES, f[u]);
+                else load_in8<F32, V16>(row, f[u]);
+            }
+            // the rows of the next turn into L2 meanwhile
+            if (g0 + U < g_hi && (at * ES & 127) == 0) {
+#pragma unroll
+                for (int u = U; u < 2 * U; u++) {
+                    const uint8_t* row = src + min((g0 + u) * RPW + sub, last) * src_step;
+                    prefetch_l2(row);
+                    if constexpr (kApart) prefetch_l2(row + a.hd / 2 * ES);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (g0 + u >= g_hi) break;
+                const int h = (g0 + u) * RPW + sub;
+                if (normed) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) sum = fmaf(f[u][j], f[u][j], sum);
+                    if (!inside) sum = 0.0f;
+#pragma unroll
+                    for (int m = LPR / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+                    const float r = rsqrtf(fmaf(sum, a.inv_hd, a.eps));
+#pragma unroll
+                    for (int j = 0; j < 8; j++) f[u][j] = f[u][j] * r * w[j];
+                }
+                if constexpr (kApart) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float x = f[u][j], y = f[u][4 + j];
+                        f[u][j] = fmaf(x, cs[j], -y * sn[j]), f[u][4 + j] = fmaf(y, cs[j], x * sn[j]);
+                    }
+                } else if constexpr (kTurn) {
+                    float other[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) other[j] = a.neox ? __shfl_sync(0xffffffffu, f[u][j], partner) : f[u][j ^ 1];
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (c + j < a.n_dims) f[u][j] = fmaf(f[u][j], cs[j], other[j] * sn[j]);
+                }
+                const bool live = h <= last && inside;
+                uint8_t* out = dst + h * dst_step;
+                if constexpr (kTensor) {
+                    if (!live) continue;
+                    if constexpr (HALVES) store_out4x2(out, c, f[u], a.hd, a.out_f32);
+                    else store_out8<V16>(out + c * (a.out_f32 ? 4 : 2), f[u], a.out_f32);
+                } else if constexpr (kApart) {
+                    store_row4x2<CACHE>(out, l, f[u], live && stored, a.hd);
+                } else {
+                    store_row8<CACHE>(out, 8 * l, f[u], live && stored, a.hd);
+                }
+            }
+        }
+    };
+    rows(std::integral_constant<int, 0>());
+    rows(std::integral_constant<int, 1>());
+    if constexpr (CACHE != B200_TYPE_F32) rows(std::integral_constant<int, 2>());
 }
 
 template <bool F32, bool V16, int CACHE>
@@ -150,9 +254,13 @@ cudaError_t launch_lanes(const RopeArgs& a, unsigned grid, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (a.hd <= 32) return cudaLaunchKernelEx(&cfg, qk_rope_kernel<F32, V16, 4, CACHE>, a);
-    if (a.hd <= 64) return cudaLaunchKernelEx(&cfg, qk_rope_kernel<F32, V16, 8, CACHE>, a);
-    return cudaLaunchKernelEx(&cfg, qk_rope_kernel<F32, V16, 16, CACHE>, a);
+    if constexpr (V16) {
+        if (a.neox && a.n_dims == a.hd && a.hd == 64) return cudaLaunchKernelEx(&cfg, qk_rope_kernel<F32, true, 8, CACHE, true>, a);
+        if (a.neox && a.n_dims == a.hd && a.hd == 128) return cudaLaunchKernelEx(&cfg, qk_rope_kernel<F32, true, 16, CACHE, true>, a);
+    }
+    if (a.hd <= 32) return cudaLaunchKernelEx(&cfg, qk_rope_kernel<F32, V16, 4, CACHE, false>, a);
+    if (a.hd <= 64) return cudaLaunchKernelEx(&cfg, qk_rope_kernel<F32, V16, 8, CACHE, false>, a);
+    return cudaLaunchKernelEx(&cfg, qk_rope_kernel<F32, V16, 16, CACHE, false>, a);
 }
 
 template <int CACHE>
@@ -232,7 +340,7 @@ int set_params(RopeArgs& a, int64_t hd, const b200_rope_params* r, const b200_te
         if ((uintptr_t)w->data % 4) return B200_E_ALIGN;
         a.w[x] = (const float*)w->data;
     }
-    a.hd = (int)hd, a.n_dims = r->n_dims, a.neox = r->mode == B200_ROPE_NEOX, a.eps = r->eps;
+    a.hd = (int)hd, a.n_dims = r->n_dims, a.neox = r->mode == B200_ROPE_NEOX, a.eps = r->eps, a.inv_hd = 1.0f / (float)hd;
     fill_turns(*r, a.turns);
     return B200_OK;
 }
