@@ -23,11 +23,32 @@ __device__ __forceinline__ uint32_t round_away(float t) {
 __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-// trunc(x * id + 8.5) clamped to [0, 15], in the low four bits: the sum is rounded towards zero, which no integer lies in the
-// way of, so the result is that of the exact sum; a second such addition leaves the integer in the low bits.  NaN gives 0.
-__device__ __forceinline__ uint32_t nibble_of(float x, float id) {
-    const float t = fminf(fmaxf(__fmaf_rz(x, id, 8.5f), 0.0f), 15.5f);
-    return (uint32_t)__float_as_int(__fadd_rz(t, 8388608.0f));
+// Four Q4_0 nibbles in the low halves of a word's bytes: trunc(x * id + 8.5), at most 15, for x * id in [-8, 8] up to a rounding.
+// The sum is formed on top of 2^22 and rounded towards zero, which leaves a whole number of halves (bit 0 of the result) and cannot
+// reach an integer that the exact sum does not reach; 16 becomes 15.  (A block with values that are no numbers gets some nibble.)
+__device__ __forceinline__ uint32_t nibbles_of(float x0, float x1, float x2, float x3, float id) {
+    constexpr float kBase = 4194304.0f + 8.5f;
+    const uint32_t w = low_bytes(__float_as_uint(__fmaf_rz(x0, id, kBase)), __float_as_uint(__fmaf_rz(x1, id, kBase)), __float_as_uint(__fmaf_rz(x2, id, kBase)),
+                                 __float_as_uint(__fmaf_rz(x3, id, kBase)));
+    const uint32_t n = (w >> 1) & 0x1F1F1F1Fu;
+    return (n - ((n >> 4) & 0x01010101u)) & 0x0F0F0F0Fu;
+}
+// Whether the first of a block's values of largest magnitude `amax` is negative.  Its values are N in each of LANES neighbouring lanes, in the
+// lanes' order, the lane's largest and smallest being hi and lo.
+template <int N, int LANES>
+__device__ __forceinline__ bool largest_is_negative(const float* x, float hi, float lo, float amax) {
+    const int base = threadIdx.x & (32 - LANES);
+    const uint32_t pos = __ballot_sync(0xffffffffu, hi == amax) >> base & ((1u << LANES) - 1), neg = __ballot_sync(0xffffffffu, lo == -amax) >> base & ((1u << LANES) - 1);
+    bool negative = neg && !pos;
+    if (__any_sync(0xffffffffu, pos && neg)) {   // both signs, or nothing but zeros
+        uint32_t sign = 0;
+#pragma unroll
+        for (int i = N - 1; i >= 0; i--)
+            if (fabsf(x[i]) == amax) sign = __float_as_uint(x[i]) >> 31;
+        sign = __shfl_sync(0xffffffffu, sign, pos | neg ? __ffs(pos | neg) - 1 : 0, LANES);
+        if (pos && neg) negative = sign;
+    }
+    return negative;
 }
 
 // Eight values f of a row, [c, c + 8), into the cache row at row_out.  All lanes of the warp call it, four neighbouring lanes
@@ -48,10 +69,15 @@ __device__ __forceinline__ void store_row8(uint8_t* row_out, int c, const float 
             *reinterpret_cast<uint4*>(row_out + c * 2) =
                 make_uint4(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]), pack_half2(f[4], f[5]), pack_half2(f[6], f[7]));
     } else {
-        float amax = 0.0f;
+        float amax = 0.0f, hi = f[0], lo = f[0];
+        if constexpr (TYPE == B200_TYPE_Q4_0) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(f[i]));
-        const float own = amax;
+            for (int i = 1; i < 8; i++) hi = fmaxf(hi, f[i]), lo = fminf(lo, f[i]);
+            amax = fmaxf(hi, -lo);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(f[i]));
+        }
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const int blk = c >> 5, i4 = (c & 31) >> 3;   // lane i4 of the block's four
@@ -84,21 +110,10 @@ __device__ __forceinline__ void store_row8(uint8_t* row_out, int c, const float 
                 if (i4 == 0) *reinterpret_cast<uint16_t*>(out) = (uint16_t)dbits;
             }
         } else {
-            // the sign of m: that of the first value of the lowest lane that has the largest magnitude
-            uint32_t sign = 0;
-#pragma unroll
-            for (int i = 7; i >= 0; i--)
-                if (fabsf(f[i]) == amax) sign = __float_as_uint(f[i]) >> 31;
-            const uint32_t has = __ballot_sync(0xffffffffu, own == amax) >> (threadIdx.x & 28) & 15u;
-            sign = __shfl_sync(0xffffffffu, sign, has ? __ffs(has) - 1 : 0, 4);
-            const float d = amax * (sign ? 0.125f : -0.125f);   // (a power of two: exact but for denormals, where d is 0 in fp16)
+            // (m / -8 is exact but for denormals, where d is 0 in fp16)
+            const float d = amax * (largest_is_negative<8, 4>(f, hi, lo, amax) ? 0.125f : -0.125f);
             const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
-            uint32_t w0 = 0, w1 = 0;
-#pragma unroll
-            for (int i = 3; i >= 0; i--) {
-                w0 = (w0 << 8) | (nibble_of(f[i], id) & 15u);
-                w1 = (w1 << 8) | (nibble_of(f[4 + i], id) & 15u);
-            }
+            const uint32_t w0 = nibbles_of(f[0], f[1], f[2], f[3], id), w1 = nibbles_of(f[4], f[5], f[6], f[7], id);
             const bool high = i4 & 2;
             const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? w0 : w1, 2);
             const uint32_t w = high ? other | (w1 << 4) : w0 | (other << 4);
@@ -128,8 +143,8 @@ __device__ __forceinline__ void store_row4x2(uint8_t* row_out, int l, const floa
             continue;
         }
         const int blk = (l >> 3) + part * (hd / 64);
-        const float own = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-        float amax = own;
+        const float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
+        float amax = fmaxf(hi, -lo);
 #pragma unroll
         for (int m = 1; m < 8; m <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, m));
         if constexpr (TYPE == B200_TYPE_Q8_0) {
@@ -147,17 +162,9 @@ __device__ __forceinline__ void store_row4x2(uint8_t* row_out, int l, const floa
                 if (i8 == 7) *reinterpret_cast<uint16_t*>(out + 4) = (uint16_t)(w >> 16);
             }
         } else if constexpr (TYPE == B200_TYPE_Q4_0) {
-            uint32_t sign = 0;
-#pragma unroll
-            for (int i = 3; i >= 0; i--)
-                if (fabsf(x[i]) == amax) sign = __float_as_uint(x[i]) >> 31;
-            const uint32_t has = __ballot_sync(0xffffffffu, own == amax) >> (threadIdx.x & 24) & 255u;
-            sign = __shfl_sync(0xffffffffu, sign, has ? __ffs(has) - 1 : 0, 8);
-            const float d = amax * (sign ? 0.125f : -0.125f);
+            const float d = amax * (largest_is_negative<4, 8>(x, hi, lo, amax) ? 0.125f : -0.125f);
             const float id = d != 0.0f ? __frcp_rn(d) : 0.0f;
-            uint32_t w = 0;
-#pragma unroll
-            for (int i = 3; i >= 0; i--) w = (w << 8) | (nibble_of(x[i], id) & 15u);
+            uint32_t w = nibbles_of(x[0], x[1], x[2], x[3], id);
             const uint32_t other = __shfl_xor_sync(0xffffffffu, w, 4);   // values 16.. of the block are lanes 4..7's
             w = i8 < 4 ? w | (other << 4) : other | (w << 4);
             if (!live) continue;
