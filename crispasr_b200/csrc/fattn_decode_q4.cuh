@@ -1,6 +1,7 @@
 // fattn_decode_q4.cuh — split-KV decode over a Q4_0 cache (included by fattn_mma.cu, which has the staging, the merge and the launch).
 //
-// At most 8 query rows per KV head, no explicit mask, no softcap.  Like the kernel over a Q8_0 cache, the keys are on the M side of
+// No explicit mask, no softcap; at most 8 query rows per CTA (9 to 16 rows of a KV head are two CTAs, the second of which finds the
+// keys in L2).  Like the kernel over a Q8_0 cache, the keys are on the M side of
 // both products (S^T = K.Q^T, O^T = V^T.P^T: a block's scale belongs to an accumulator row of the thread that loaded it, or rides
 // on P), every warp copies the raw bytes of its own 16 keys of a tile and there is no barrier in the key loop.  What four bits change:
 //
@@ -57,9 +58,10 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
     __shared__ __align__(8) uint64_t s_bar[NW][NS];      // one barrier per (warp, stage)
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+    const int all_rows = a.Tq * a.gqa;   // <= 16; row rr -> (iq = rr / gqa, head hk*gqa + rr % gqa)
+    const int pair = !FEW && all_rows > 8, split = blockIdx.x, hk = blockIdx.y >> pair, b = blockIdx.z;
     const int bk = b / a.bq;
-    const int R = a.Tq * a.gqa;  // <= 8 (FEW: <= 4); row rr -> (iq = rr / gqa, head hk*gqa + rr % gqa)
+    const int row0 = pair ? 8 * (blockIdx.y & 1) : 0, R = min(8, all_rows - row0);   // this CTA's rows (FEW: <= 4)
     const float ninf = -INFINITY;
     cluster_announce(a);
 
@@ -86,7 +88,7 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
     const int q_src = FEW ? q_row & 3 : q_row;   // FEW: columns 4..7 repeat rows 0..3
     if (q_row < 8 && q_src < R) {
         int iq, hq;
-        row_to_query(a, hk, q_src, iq, hq);
+        row_to_query(a, hk, row0 + q_src, iq, hq);
         const uint8_t* rowp = a.q.p + (int64_t)iq * a.q.nb1 + (int64_t)hq * a.q.nb2 + (int64_t)b * a.q.nb3;
         if (q_f32) {
             q_val = load_global(reinterpret_cast<const uint4*>(rowp) + 2 * q_ch);
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
     const float c = a.scale * kLog2e * 512.0f;   // (quants enter as 2^-9 of themselves)
     int last[2];   // the last key that the thread's rows see
 #pragma unroll
-    for (int j = 0; j < 2; j++) last[j] = a.causal ? min(len_b - 1, n_past + (FEW ? (2 * t + j) & 3 : 2 * t + j) / a.gqa) : len_b - 1;
+    for (int j = 0; j < 2; j++) last[j] = a.causal ? min(len_b - 1, n_past + (FEW ? (2 * t + j) & 3 : row0 + 2 * t + j) / a.gqa) : len_b - 1;
 
     float top = kTop;
     float m_run[2] = {ninf, ninf}, l_run[2] = {0.0f, 0.0f};   // reference (running maximum - top) and sum of rows 2t, 2t+1; the same on the lanes that share t
@@ -360,5 +362,5 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
         }
     }
     __syncthreads();
-    decode_write_out<HD, NW, 8, FEW>(a, slab, s_m, s_l, sRaw + NW * NS * 2 * RAW, R, b, hk, split, tq_b, tid);
+    decode_write_out<HD, NW, 8, FEW>(a, slab, s_m, s_l, sRaw + NW * NS * 2 * RAW, R, b, hk, split, tq_b, tid, row0);
 }

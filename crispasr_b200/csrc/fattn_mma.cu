@@ -425,7 +425,7 @@ enum DecodeMode {
     kDecAsyncF16 = 1,  // cp.async 16-byte copies of F16 rows into a multi-stage ring
     kDecAsyncQ8 = 2,   // bulk copy of the raw Q8_0 byte range of a tile, then a shared-to-shared dequantise (head_dim 32)
     kDecRegQ8 = 3,     // bulk copy of the raw Q8_0 bytes, dequantised in registers (head_dim 64 / 128)
-    kDecRegQ4 = 4      // the same over a Q4_0 cache (head_dim 64 / 128, at most 8 query rows, no mask, no softcap)
+    kDecRegQ4 = 4      // the same over a Q4_0 cache (head_dim 64 / 128, no mask, no softcap)
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
@@ -672,11 +672,11 @@ __host__ __device__ constexpr size_t cluster_push_bytes(int hd, int rows) { retu
 // A CTA with two or three tiles shares its SM with few others, but at the usual 256-stream size three neighbours are
 // in their key loops and every dependent step of a tail waits for an issue slot, so the chain is kept short: no
 // separate pass for the common maximum, no index division per element.
-// PAIR: a query row's partial is the sum of slab rows rr and rr + 4.
+// PAIR: a query row's partial is the sum of slab rows rr and rr + 4.  row0: the KV head's query row that is row 0 of this CTA.
 template <int HD, int NW = 4, int ROWS = kDecRows, bool PAIR = false>
 __device__ __forceinline__ void decode_write_out(const FattnArgs& a, const float* slab, const float (*s_m)[kDecRows],
                                                  const float (*s_l)[kDecRows], uint8_t* recv, int R, int b, int hk, int split,
-                                                 int tq_b, int tid) {
+                                                 int tq_b, int tid, int row0 = 0) {
     constexpr int STRIDE = HD + 4, G = HD / 4;
     const float ninf = -INFINITY;
     const bool push = a.n_splits > 1 && a.cluster_merge;
@@ -706,7 +706,7 @@ __device__ __forceinline__ void decode_write_out(const FattnArgs& a, const float
         }
         if (a.n_splits == 1) {
             int iq, hq;
-            row_to_query(a, hk, rr, iq, hq);
+            row_to_query(a, hk, row0 + rr, iq, hq);
             const float inv = (L > 0.0f && iq < tq_b) ? 1.0f / L : 0.0f;
             float* drow = a.dst + (((int64_t)b * a.Tq + iq) * a.dst_heads + hq) * a.hd;
             if (a.hd == HD && (HD > 32 || (reinterpret_cast<uintptr_t>(drow) & 15) == 0)) {   // (head_dim 32 has no rule on the result's alignment)
@@ -723,8 +723,8 @@ __device__ __forceinline__ void decode_write_out(const FattnArgs& a, const float
             if (cg < a.n_splits) st_peer_v2(peer_addr(recv_ml + split * kDecRows + rr, cg), M, L);
         } else {
             const int64_t unit = ((int64_t)b * a.Hkv + hk) * a.n_splits + split;
-            *reinterpret_cast<float4*>(a.ws_o + unit * kDecRows * HD + rr * HD + 4 * cg) = v;   // live rows only: the merge kernel reads no others
-            if (cg == 0) a.ws_ml[(unit * kDecRows + rr) * 2] = M, a.ws_ml[(unit * kDecRows + rr) * 2 + 1] = L;
+            *reinterpret_cast<float4*>(a.ws_o + unit * kDecRows * HD + (row0 + rr) * HD + 4 * cg) = v;   // live rows only: the merge kernel reads no others
+            if (cg == 0) a.ws_ml[(unit * kDecRows + row0 + rr) * 2] = M, a.ws_ml[(unit * kDecRows + row0 + rr) * 2 + 1] = L;
         }
     }
     if (push) {
@@ -752,7 +752,7 @@ __device__ __forceinline__ void decode_write_out(const FattnArgs& a, const float
                 }
             }
             int iq, hq;
-            row_to_query(a, hk, rr, iq, hq);
+            row_to_query(a, hk, row0 + rr, iq, hq);
             const float inv = (L > 0.0f && iq < tq_b) ? 1.0f / L : 0.0f;
             *reinterpret_cast<float4*>(a.dst + (((int64_t)b * a.Tq + iq) * a.dst_heads + hq) * HD + 4 * cg) =
                 make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);   // the cluster form is offered for a.hd == HD only
@@ -1917,13 +1917,15 @@ bool cluster_merge_enabled() {
 // Clusters of the Q4_0 kernel find no place on the last SMs of a nearly full grid: 4 streams x 20 KV heads, 1500 keys, 480 CTAs in clusters of
 // six 6.9 us, 560 in clusters of seven 10.4.
 constexpr double kQ4ClusterFill = 0.87;
+// CTAs of the Q4_0 kernel that share a KV head's keys, eight query rows each; the other kernels take all rows in one.
+int q4_row_groups(const FattnArgs& a);
 
 bool use_cluster_merge(const FattnArgs& a) {
     // only while the whole grid is resident at once (2 to 4 CTAs on each of 148 SMs): with several waves the cluster
     // barriers hold finished CTAs on their SMs and the form measured 10 % slower than the merge kernel.  Pairs at head_dim 64 over an F16
     // cache hold little and save the merge kernel (32 segments of the large decoder 101.6 -> 97.5 us per layer).
     return decode_cluster_merge_ok(a) && a.n_splits > 1 && a.n_splits <= 8 && ((a.n_splits == 2 && a.k.type == B200_TYPE_F16 && a.hd == 64) ||
-           (long)a.n_splits * a.Hkv * a.B <= (long)decode_ctas_per_sm(a, true) * 148 * (a.k.type == B200_TYPE_Q4_0 ? kQ4ClusterFill : 1.0));
+           (long)a.n_splits * a.Hkv * a.B * q4_row_groups(a) <= (long)decode_ctas_per_sm(a, true) * 148 * (a.k.type == B200_TYPE_Q4_0 ? kQ4ClusterFill : 1.0));
 }
 
 template <typename Kern>
@@ -2057,7 +2059,8 @@ int decode_mode(const FattnArgs& a, int hdp) {
             return (a.hd == 64 || a.hd == 128) ? kDecRegQ8 : kDecAsyncQ8;
     }
     // Q4_0: rows that follow one another, from any 4-byte boundary on
-    if (a.k.type == B200_TYPE_Q4_0 && (a.hd == 64 || a.hd == 128) && !a.kv_index && !a.has_mask && a.softcap == 0.0f && a.Tq * a.gqa <= 8) {
+    if (a.k.type == B200_TYPE_Q4_0 && (a.hd == 64 || a.hd == 128) && !a.kv_index && !a.has_mask && a.softcap == 0.0f &&
+        (a.Tq * a.gqa <= 8 || a.Hkv <= 32767)) {   // (twice the CTAs along one grid dimension)
         const int64_t rb = a.hd / 32 * 18;
         const auto words = [](const View& x) { return ((uintptr_t)x.p | (uintptr_t)x.nb2 | (uintptr_t)x.nb3) % 4 == 0; };
         if (a.k.nb1 == rb && a.v.nb1 == rb && words(a.k) && words(a.v)) return kDecRegQ4;
@@ -2065,6 +2068,7 @@ int decode_mode(const FattnArgs& a, int hdp) {
     return kDecSync;
 }
 
+int q4_row_groups(const FattnArgs& a) { return a.k.type == B200_TYPE_Q4_0 && a.Tq * a.gqa > 8 && decode_mode(a, a.hd) == kDecRegQ4 ? 2 : 1; }
 size_t q4_smem(int hd, int nw) { return (size_t)8 * hd * sizeof(__half) + (size_t)kDecQ4Stages * nw * 2 * (kDecQ4Keys * (hd / 32 * 18) + kDecQ4Skew); }
 
 // The keys-on-M kernel: at most 8 query rows, plain form.
@@ -2114,10 +2118,10 @@ int launch_decode_q8reg(const FattnArgs& a, cudaStream_t st) {
 
 template <int HD>
 int launch_decode_q4(const FattnArgs& a, cudaStream_t st) {
-    dim3 grid(a.n_splits, a.Hkv, a.B);
+    dim3 grid(a.n_splits, a.Hkv * q4_row_groups(a), a.B);
     cudaError_t e;
     auto go = [&](auto kern, int nw, bool (&smem_set)[64]) {
-        const size_t main = q4_smem(HD, nw), push = use_cluster_merge(a) ? cluster_push_bytes(HD, a.Tq * a.gqa) : 0;
+        const size_t main = q4_smem(HD, nw), push = use_cluster_merge(a) ? cluster_push_bytes(HD, a.Tq * a.gqa < 8 ? a.Tq * a.gqa : 8) : 0;
         e = set_smem_once(kern, main + cluster_push_bytes(HD, 8), smem_set);
         if (e == cudaSuccess) launch_split(kern, grid, main + push, st, a, 32 * nw);
     };
@@ -2360,7 +2364,7 @@ int decode_ctas_per_sm(const FattnArgs& a, bool cluster) {
             smem = (size_t)kDecRows * hdp * 2 + (size_t)kDecRegStages * 2 * kDecBN * (hdp / 32 * 34);
             break;
         case kDecRegQ4: {
-            smem = q4_smem(hdp, a.wide ? 8 : 4) + (cluster ? cluster_push_bytes(hdp, a.Tq * a.gqa) : 0);
+            smem = q4_smem(hdp, a.wide ? 8 : 4) + (cluster ? cluster_push_bytes(hdp, a.Tq * a.gqa < 8 ? a.Tq * a.gqa : 8) : 0);
             const int n = (int)((size_t)227 * 1024 / (smem + 1536 + 1024)), most = a.wide ? 2 : 4;
             return n < 1 ? 1 : (n > most ? most : n);
         }
@@ -2396,7 +2400,7 @@ void decode_split_force(int n_splits) { g_forced_splits.store(n_splits, std::mem
 // units (78.8 us against 75.5 in two splits).  Eight warps: 8 streams x 2000 keys 10.6 -> 10.0 us, one of 4000 7.9 -> 6.6, 16 of 535 9.1 -> 6.8.
 int q4_choose(FattnArgs& a, int B, int sm_count) {
     const int Lk = a.Lk;
-    const double units = (double)B * a.Hkv, f = a.hd == 128 ? 1.0 : 0.55;
+    const double units = (double)B * a.Hkv * q4_row_groups(a), f = a.hd == 128 ? 1.0 : 0.55;
     constexpr double kStep[5] = {0.0, 1.0, 1.5, 2.0, 2.45};
     int best = 1;
     double best_cost = 0.0;

@@ -428,3 +428,24 @@ def test_serving_form_on_word_boundaries(b200, shift):
         q = randn_f16(rng, (2, 6, 1, hd))
         got = gpu_op(b200, q, cuda_view(base[shift:].reshape(k.shape), base), v, scale=0.1, kv_type=abi.Q4_0)
         _exact(got, attention_f64(q, kf, vf, 0.1), f"{hd} {L}")
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("gqa,Tq", [(4, 4), (1, 9), (2, 8), (3, 5), (13, 1)])
+@pytest.mark.parametrize("splits", [0, 2, 7, 20])
+def test_nine_to_sixteen_rows(b200, hd, gqa, Tq, splits):
+    """A KV head's rows in two CTAs: plain, causal with ragged row counts, a scalar bound, every form of the merge."""
+    rng = np.random.default_rng(hd + gqa + Tq + splits)
+    B, Hkv, L = 3, 2, 1700
+    k, v, kf, vf = _caches(rng, B, Hkv, L, hd)
+    q = randn_f16(rng, (B, Hkv * gqa, Tq, hd))
+    lens = np.array([L, 0, 777], np.int32)
+    forms = [dict(kv_len=lens), dict(kv_len=lens, q_len=np.array([Tq, 0, max(1, Tq - 2)], np.int32), causal=True), dict(causal=True, n_past=L - Tq - 5)]
+    assert b200.lib().b200_set_decode_splits(splits) == 0
+    try:
+        for kw in forms:
+            got = gpu_op(b200, q, k, v, scale=hd ** -0.5, kv_type=abi.Q4_0, **kw)
+            assert b200.lib().b200_last_kernel() == abi.KERNEL_DECODE_SPLIT
+            _exact(got, attention_f64(q, kf, vf, hd ** -0.5, **kw), str(kw.keys()))
+    finally:
+        b200.lib().b200_set_decode_splits(0)
