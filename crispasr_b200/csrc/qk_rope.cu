@@ -390,6 +390,7 @@ B200_API int b200_kv_append_rope(b200_kv_cache* kv, int layer, const b200_tensor
                                  const int32_t* n_rows, const b200_tensor* q_out, void* cuda_stream) {
     if (!kv || !k_new || !v_new || (q == nullptr) != (q_out == nullptr)) return B200_E_NULL;
     if (layer < 0 || layer >= kv->cfg.n_layers) return B200_E_SHAPE;
+    if (!on_current_device(kv)) return B200_E_STATE;
     RopeArgs a = {};
     Alignment al;
     int rc;

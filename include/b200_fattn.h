@@ -31,6 +31,11 @@
  * type); K/V quantised blocks are dequantised as fp32(d) * q (Q8_0) or
  * fp32(d) * (q - 8) (Q4_0: value i of a block in the low nibble of byte i,
  * value 16 + i in the high one).  A row whose keys are all masked yields zeros.
+ *
+ * Accuracy: operands of the tensor cores are F16, the weights P among them (relative 2^-11 each).  Decode over a Q4_0 cache
+ * (head_dim 64 / 128, Tq * (H / Hkv) <= 16, no mask, softcap or index list, rows that follow one another from a 4-byte boundary on)
+ * keeps P and the products to fp32: relative L2 below 2^-17.  Its rows at or beyond kv_len may hold anything; a key that only the
+ * causal bound hides from a row has to be finite.
  */
 #ifndef B200_FATTN_H
 #define B200_FATTN_H
@@ -331,7 +336,8 @@ B200_API int b200_kv_view(const b200_kv_cache* kv, int layer, int64_t n_rows, b2
  * write branch at :840-867 (ggml_cpy for F16, ggml_set_rows for quantised caches): converts
  * F32 rows k_new/v_new [hd, n_new, n_kv_heads, n_streams] (device, generic strides) to the cache
  * type and stores them at rows pos[s] .. pos[s]+n_new-1 of each stream s (`pos` is a device
- * array [n_streams], or NULL meaning `pos0` for all).  Asynchronous on `cuda_stream`.
+ * array [n_streams], or NULL meaning `pos0` for all).  A Q4_0 block's scale is its value of largest magnitude (the first
+ * of them) / -8, its nibbles trunc(x / scale + 8.5), at most 15.  Asynchronous on `cuda_stream`.
  */
 B200_API int b200_kv_append(b200_kv_cache* kv, int layer, const b200_tensor* k_new, const b200_tensor* v_new,
                             const int32_t* pos, int32_t pos0, void* cuda_stream);
@@ -340,7 +346,8 @@ B200_API int b200_kv_append(b200_kv_cache* kv, int layer, const b200_tensor* k_n
  * runtimes read a quantised cache (src/core/attention.h:887-920), for callers that move a stream to a cache of another
  * type, keep it on the host or feed an operator of their own.  k_out/v_out are F32 or F16 (both the same)
  * [hd, n, n_kv_heads, n_streams] on the device, generic strides; row i of stream s is cache row pos[s] + i (`pos0` + i where
- * `pos` is NULL), rows outside the cache read as zeros.  Asynchronous on `cuda_stream`.
+ * `pos` is NULL), rows outside the cache read as zeros.  The cache's device has to be the current one (else B200_E_STATE).
+ * Asynchronous on `cuda_stream`.
  */
 B200_API int b200_kv_read(const b200_kv_cache* kv, int layer, const b200_tensor* k_out, const b200_tensor* v_out,
                           const int32_t* pos, int32_t pos0, void* cuda_stream);
@@ -368,7 +375,8 @@ typedef struct b200_rope_params {
 /*
  * b200_qk_norm_rope — norm and rotation alone, for callers with caches of their own.  q [hd, n, H, S] and k [hd, n, Hkv, S]
  * (k and k_out may be NULL) are F32 or F16 (both the same), device, generic strides, hd a multiple of 8 up to 128; q_out and
- * k_out have their shapes and are F32 or F16 (both the same); an output may be its input.  q_norm / k_norm: F32 [hd] weights,
+ * k_out have their shapes and are F32 or F16 (both the same); an output may be its input, and overlaps nothing else that the call
+ * reads or writes.  q_norm / k_norm: F32 [hd] weights,
  * or NULL (no norm).  Row i of stream s is at position pos[s] + i (`pos` a device array [S], or NULL meaning `pos0` for all).
  * n_rows: device array [S] of valid rows per stream, or NULL; output rows at or beyond it are zeros.  Asynchronous on
  * `cuda_stream`.
@@ -380,7 +388,7 @@ B200_API int b200_qk_norm_rope(const b200_tensor* q, const b200_tensor* k, const
  * b200_kv_append_rope — the same for q (to q_out; both may be NULL) and k_new, and k_new and v_new converted to the cache
  * type and stored at rows pos[s] .. of every stream, as b200_kv_append stores them; the position of a row is its place in
  * the cache.  q, k_new and v_new are all F32 or all F16.  Rows at or beyond n_rows[s], and rows outside the cache, are not
- * stored.
+ * stored.  The cache's device has to be the current one (else B200_E_STATE).
  */
 B200_API int b200_kv_append_rope(b200_kv_cache* kv, int layer, const b200_tensor* q, const b200_tensor* k_new, const b200_tensor* v_new,
                                  const b200_tensor* q_norm, const b200_tensor* k_norm, const b200_rope_params* params,
