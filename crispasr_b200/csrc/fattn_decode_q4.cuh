@@ -123,6 +123,8 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
         if (key0 + i * KT < key_end) issue(key0 + i * KT, i);
     if (q_f32) q_val = f32x8_to_half(q_val, q_hi);
     if (q_row < 8) {
+        // rows behind q_len may hold anything: their result is a zero times what comes of them
+        if ((row0 + q_src) / a.gqa >= tq_b) q_val = make_uint4(0u, 0u, 0u, 0u);
         const int blk = q_ch >> 2;
         const __half* h = reinterpret_cast<const __half*>(&q_val);
         // value 16 ks + j of a block to the place where the quad's thread that has byte j finds it: even blocks bytes 2 + 4t .. 5 + 4t
@@ -348,8 +350,11 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
         lq[j] = v;
     }
     if (g == 0) {
-        s_m[warp][2 * t] = m_run[0], s_m[warp][2 * t + 1] = m_run[1];
-        s_l[warp][2 * t] = lq[0], s_l[warp][2 * t + 1] = lq[1];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {   // (scores that are no numbers raise no maximum: the row must not pass for one without keys)
+            s_m[warp][2 * t + j] = lq[j] == lq[j] ? m_run[j] : 0.0f;
+            s_l[warp][2 * t + j] = lq[j];
+        }
     }
     __syncthreads();  // the warps' (m, l) are visible, and all warps are done with the raw stages (the merge slabs alias them)
 #pragma unroll

@@ -449,3 +449,67 @@ def test_nine_to_sixteen_rows(b200, hd, gqa, Tq, splits):
             _exact(got, attention_f64(q, kf, vf, hd ** -0.5, **kw), str(kw.keys()))
     finally:
         b200.lib().b200_set_decode_splits(0)
+
+
+@pytest.mark.parametrize("gqa,Tq", [(1, 4), (2, 4), (4, 4)])
+def test_query_rows_behind_their_count_may_hold_anything(b200, gqa, Tq):
+    """NaN and infinities in padding rows of Q: zeros there, and nothing of them in the other rows."""
+    rng = np.random.default_rng(gqa)
+    B, Hkv, L, hd = 3, 2, 140, 128
+    k, v, kf, vf = _caches(rng, B, Hkv, L, hd)
+    q = randn_f16(rng, (B, Hkv * gqa, Tq, hd))
+    q_len, kv_len = np.array([1, 0, 3], np.int32), np.array([140, 9, 77], np.int32)
+    for b in range(B):
+        q[b, :, q_len[b]:] = np.nan
+        q[b, ::2, q_len[b]:] = np.inf
+    for causal in (False, True):
+        kw = dict(scale=0.1, kv_len=kv_len, q_len=q_len, causal=causal)
+        got = gpu_op(b200, q, k, v, kv_type=abi.Q4_0, **kw)
+        for b in range(B):
+            assert not got[b, q_len[b]:].any()
+        _exact(got, attention_f64(q, kf, vf, **kw), "padding rows")
+
+
+def test_a_query_that_is_no_number_stays_by_itself(b200):
+    """A row of NaN gives NaN, the rows that share its keys and its CTA do not change."""
+    rng = np.random.default_rng(77)
+    k, v, kf, vf = _caches(rng, 1, 2, 300, 128)
+    q = randn_f16(rng, (1, 8, 1, 128))
+    want = gpu_op(b200, q, k, v, scale=0.1, kv_type=abi.Q4_0)
+    q[0, 2, 0, 5] = np.nan
+    got = gpu_op(b200, q, k, v, scale=0.1, kv_type=abi.Q4_0)
+    assert np.isnan(got[0, 0, 2]).all()
+    keep = [h for h in range(8) if h != 2]
+    assert np.array_equal(got[0, 0, keep], want[0, 0, keep])
+
+
+def test_two_streams_and_two_graphs_at_once(b200):
+    """Launches with splits of their own on two streams, and two graphs of different lengths over one cache replayed in turn."""
+    rng = np.random.default_rng(5)
+    k, v, kf, vf = _caches(rng, 1, 8, 5000, 128)
+    dk, dv = torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda()
+    qs = [torch.from_numpy(randn_f16(rng, (1, 32, 1, 128))).cuda() for _ in range(2)]
+    lens = [torch.tensor([n], dtype=torch.int32, device="cuda") for n in (5000, 1234)]
+    streams, outs, graphs = [torch.cuda.Stream() for _ in range(2)], [None, None], []
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i] = b200.flash_attn_ext(qs[i], dk, dv, scale=0.1, kv_type=abi.Q4_0, kv_len=lens[i])
+    torch.cuda.synchronize()
+    for i in range(2):
+        ref = attention_f64(qs[i].cpu().numpy(), kf, vf, 0.1, kv_len=lens[i].cpu().numpy())
+        _exact(outs[i].cpu().numpy(), ref, f"stream {i}")
+    held = []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(b200.flash_attn_ext(qs[i], dk, dv, scale=0.1, kv_type=abi.Q4_0, kv_len=lens[i]))
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(held[i], outs[i])
+    assert b200.lib().b200_device_status() == 0
