@@ -15,6 +15,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/b200_fattn.h"
@@ -397,7 +398,7 @@ PyObject* kv_append_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // The arguments of the rotation's calls; all by keyword, unknown names are an error.
 enum RopeKey { rQNorm, rKNorm, rEps, rDims, rBase, rScale, rNeox, rPos, rPos0, rNRows, rOut, rKOut, rStream, rKeys };
 const char* const kRopeNames[rKeys] = {"q_norm", "k_norm", "eps", "rope_dims", "rope_base", "rope_scale", "neox", "pos", "pos0", "n_rows", "out", "k_out", "stream"};
-PyObject* g_rope_keys[rKeys];
+PyObject *g_rope_keys[rKeys], *g_handle, *g_value;
 
 // An int32 table on the device of `like`, one entry per stream.
 bool table_of(PyObject* o, const char* what, const at::Tensor& like, int64_t streams, const int32_t** out) {
@@ -552,14 +553,33 @@ PyObject* qk_norm_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObject*
     END_HANDLE_TH_ERRORS
 }
 
-// (cache address, layer, q, k_new, v_new, *, ...)
+// The address in a KvCache object (its `_h`, a ctypes pointer; null after close()).
+bool cache_of(PyObject* self, b200_kv_cache** out) {
+    PyObject* h = PyObject_GetAttr(self, g_handle);
+    PyObject* value = h ? PyObject_GetAttr(h, g_value) : nullptr;
+    Py_XDECREF(h);
+    if (!value) return false;
+    *out = value == Py_None ? nullptr : (b200_kv_cache*)PyLong_AsVoidPtr(value);
+    Py_DECREF(value);
+    return !PyErr_Occurred();
+}
+
+const char kAppendRopeDoc[] =
+    "append_rope(self, layer, q, k_new, v_new, *, q_norm=None, k_norm=None, eps=1e-6, rope_dims=head_dim, rope_base=10000.0, rope_scale=1.0,\n"
+    "            neox=True, pos=None, pos0=0, n_rows=None, out=None, stream=None)\n--\n\n"
+    "Norm (where a weight is given) and rotation of q (n_streams, heads, n_new, hd; or None) and k_new (n_streams, n_kv, n_new, hd), and\n"
+    "k_new and v_new into the cache.  All float32 or all float16 CUDA tensors.  Row i of stream s is at position pos[s] + i, which is\n"
+    "also its place in the cache; the other arguments as in qk_norm_rope.  Returns the rotated q, float16 unless `out` says otherwise.";
+
+// A method of KvCache: called with the object in front.
 PyObject* kv_append_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObject* names) {
     HANDLE_TH_ERRORS
     if (n != 5) {
         PyErr_SetString(PyExc_TypeError, "append_rope() takes 4 positional arguments (layer, q, k_new, v_new)");
         return nullptr;
     }
-    b200_kv_cache* kv = (b200_kv_cache*)PyLong_AsVoidPtr(a[0]);
+    b200_kv_cache* kv = nullptr;
+    if (!cache_of(a[0], &kv)) return nullptr;
     const long layer = PyLong_AsLong(a[1]);
     if (PyErr_Occurred()) return nullptr;
     RopeCall call;
@@ -627,20 +647,53 @@ PyObject* kv_tensors_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// (cache address, layer, n_rows, pos, pos0, f32, out, stream): K and V rows as values
-PyObject* kv_read_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    if (n != 8) {
-        PyErr_SetString(PyExc_TypeError, "kv_read takes 8 arguments");
+const char kReadDoc[] =
+    "read(self, layer, n_rows, pos=None, pos0=0, dtype=None, out=None, stream=None)\n--\n\n"
+    "Rows pos[s] .. pos[s] + n_rows - 1 of every stream (`pos` an int32 CUDA tensor, else `pos0` for all) as values: (K, V), each\n"
+    "(n_streams, n_kv, n_rows, hd) float16, or float32 if `dtype` says so, or the pair `out`.  Rows outside the cache are zeros.";
+
+// A method of KvCache: called with the object in front.
+PyObject* kv_read_py(PyObject*, PyObject* const* in, Py_ssize_t n, PyObject* names) {
+    HANDLE_TH_ERRORS
+    enum { kLayer, kRows, kPos, kPos0, kDtype, kOutPair, kOn, kArgs };
+    static const char* const arg_names[kArgs] = {"layer", "n_rows", "pos", "pos0", "dtype", "out", "stream"};
+    PyObject* a[kArgs] = {};
+    if (n < 1 || n > kArgs + 1) {
+        PyErr_SetString(PyExc_TypeError, "read() takes from 2 to 7 arguments");
         return nullptr;
     }
-    HANDLE_TH_ERRORS
-    const b200_kv_cache* kv = (const b200_kv_cache*)PyLong_AsVoidPtr(a[0]);
-    const long layer = PyLong_AsLong(a[1]), rows = PyLong_AsLong(a[2]), pos0 = PyLong_AsLong(a[4]);
-    const int f32 = PyObject_IsTrue(a[5]);
-    if (PyErr_Occurred()) return nullptr;
-    if (pos0 != (int32_t)pos0) {
-        PyErr_SetString(PyExc_OverflowError, "pos0 is a 32-bit number");
+    for (Py_ssize_t i = 1; i < n; i++) a[i - 1] = in[i];
+    for (Py_ssize_t j = 0; j < (names ? PyTuple_GET_SIZE(names) : 0); j++) {
+        int hit = -1;
+        for (int i = 0; i < kArgs && hit < 0; i++)
+            if (PyUnicode_CompareWithASCIIString(PyTuple_GET_ITEM(names, j), arg_names[i]) == 0) hit = i;
+        if (hit < 0 || a[hit]) {
+            PyErr_Format(PyExc_TypeError, hit < 0 ? "read() got an unexpected keyword argument '%U'" : "read() got multiple values for argument '%U'",
+                         PyTuple_GET_ITEM(names, j));
+            return nullptr;
+        }
+        a[hit] = in[n + j];
+    }
+    if (!a[kLayer] || !a[kRows]) {
+        PyErr_SetString(PyExc_TypeError, "read() needs layer and n_rows");
         return nullptr;
+    }
+    for (PyObject*& x : a)
+        if (x == Py_None) x = nullptr;
+    b200_kv_cache* kv = nullptr;
+    if (!cache_of(in[0], &kv)) return nullptr;
+    const long layer = a[kLayer] ? PyLong_AsLong(a[kLayer]) : -1, rows = a[kRows] ? PyLong_AsLong(a[kRows]) : -1, pos0 = a[kPos0] ? PyLong_AsLong(a[kPos0]) : 0;
+    if (PyErr_Occurred()) return nullptr;
+    if (pos0 != (int32_t)pos0 || layer != (int32_t)layer) {
+        PyErr_SetString(PyExc_OverflowError, "layer and pos0 are 32-bit numbers");
+        return nullptr;
+    }
+    at::ScalarType type = at::kHalf;
+    if (a[kDtype]) {
+        if (!THPDtype_Check(a[kDtype]) || ((type = ((THPDtype*)a[kDtype])->scalar_type) != at::kHalf && type != at::kFloat)) {
+            PyErr_SetString(PyExc_ValueError, "dtype is torch.float16 or torch.float32");
+            return nullptr;
+        }
     }
     b200_tensor view[2], t[2];
     int rc = b200_kv_view(kv, (int)layer, rows, &view[0], &view[1]);
@@ -649,16 +702,16 @@ PyObject* kv_read_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(device);
     const int64_t sizes[4] = {view[0].ne[3], view[0].ne[2], rows, view[0].ne[0]};
     at::Tensor out[2];
-    if (a[6] == Py_None) {
-        for (at::Tensor& o : out) o = at::detail::empty_cuda(sizes, f32 ? at::kFloat : at::kHalf, device, std::nullopt);
+    if (!a[kOutPair]) {
+        for (at::Tensor& o : out) o = at::detail::empty_cuda(sizes, type, device, std::nullopt);
     } else {
-        if (!PyTuple_Check(a[6]) || PyTuple_GET_SIZE(a[6]) != 2) {
+        if (!PyTuple_Check(a[kOutPair]) || PyTuple_GET_SIZE(a[kOutPair]) != 2) {
             PyErr_SetString(PyExc_TypeError, "out is a pair of tensors");
             return nullptr;
         }
         for (int i = 0; i < 2; i++) {
             const at::Tensor* o = nullptr;
-            if (!rows_of(PyTuple_GET_ITEM(a[6], i), "out", nullptr, &o)) return nullptr;
+            if (!rows_of(PyTuple_GET_ITEM(a[kOutPair], i), "out", nullptr, &o)) return nullptr;
             if (o->device() != device || o->size(2) != rows) {
                 PyErr_SetString(PyExc_ValueError, "out has n_rows rows and is on the cache's device");
                 return nullptr;
@@ -668,10 +721,10 @@ PyObject* kv_read_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     if (!describe(out[0], -1, &t[0]) || !describe(out[1], -1, &t[1])) return nullptr;
     const int32_t* pos = nullptr;
-    if (a[3] != Py_None && !table_of(a[3], "pos", out[0], sizes[0], &pos)) return nullptr;
+    if (a[kPos] && !table_of(a[kPos], "pos", out[0], sizes[0], &pos)) return nullptr;
     void* st = nullptr;
-    if (a[7] == Py_None) st = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-    else if (!stream_of(a[7], &st)) return nullptr;
+    if (!a[kOn]) st = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    else if (!stream_of(a[kOn], &st)) return nullptr;
     Py_BEGIN_ALLOW_THREADS
     rc = b200_kv_read(kv, (int)layer, &t[0], &t[1], pos, (int32_t)pos0, st);
     Py_END_ALLOW_THREADS
@@ -685,14 +738,17 @@ PyObject* kv_read_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+PyObject* as_method_py(PyObject*, PyObject* function) { return PyInstanceMethod_New(function); }
+
 PyMethodDef kMethods[] = {
     {"flash_attn_ext", (PyCFunction)(void (*)(void))launch_py, METH_FASTCALL | METH_KEYWORDS, kLaunchDoc},
     {"flash_attn_ext_host", (PyCFunction)(void (*)(void))forward_host_py, METH_FASTCALL | METH_KEYWORDS, kHostDoc},
     {"kv_append", (PyCFunction)(void (*)(void))kv_append_py, METH_FASTCALL, "rows of a KV cache"},
     {"qk_norm_rope", (PyCFunction)(void (*)(void))qk_norm_rope_py, METH_FASTCALL | METH_KEYWORDS, kQkRopeDoc},
-    {"kv_append_rope", (PyCFunction)(void (*)(void))kv_append_rope_py, METH_FASTCALL | METH_KEYWORDS, "norm, rotation and rows of a KV cache"},
+    {"kv_append_rope", (PyCFunction)(void (*)(void))kv_append_rope_py, METH_FASTCALL | METH_KEYWORDS, kAppendRopeDoc},
     {"kv_tensors", (PyCFunction)(void (*)(void))kv_tensors_py, METH_FASTCALL, "views of a KV cache"},
-    {"kv_read", (PyCFunction)(void (*)(void))kv_read_py, METH_FASTCALL, "rows of a KV cache as values"},
+    {"kv_read", (PyCFunction)(void (*)(void))kv_read_py, METH_FASTCALL | METH_KEYWORDS, kReadDoc},
+    {"method", as_method_py, METH_O, "the function as one that binds to an object as a method (a built-in function does not)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_op", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
@@ -701,6 +757,7 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_op", nullptr, -1, kMethods
 PyMODINIT_FUNC PyInit__torch_op(void) {
     for (int i = 0; i < kKeys; i++)
         if (!(g_keys[i] = PyUnicode_InternFromString(kKeyNames[i]))) return nullptr;
+    if (!(g_handle = PyUnicode_InternFromString("_h")) || !(g_value = PyUnicode_InternFromString("value"))) return nullptr;
     for (int i = 0; i < rKeys; i++)
         if (!(g_rope_keys[i] = PyUnicode_InternFromString(kRopeNames[i]))) return nullptr;
     return PyModule_Create(&kModule);

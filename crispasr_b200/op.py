@@ -106,6 +106,8 @@ def workspace_bytes(q, k, v, mask=None, **kw) -> int:
 # of its functions: the rest of the package needs none.
 _NATIVE = {"flash_attn_ext": "flash_attn_ext", "flash_attn_ext_host": "flash_attn_ext_host", "qk_norm_rope": "qk_norm_rope", "_kv_append": "kv_append",
            "_kv_append_rope": "kv_append_rope", "_kv_tensors": "kv_tensors", "_kv_read": "kv_read"}
+# ... and methods of KvCache are they themselves, once loaded: a Python function in front, passing keywords on, costs 0.6 us a call
+_METHODS = {"append_rope": "_kv_append_rope", "read": "_kv_read"}
 
 
 def _load_native():
@@ -114,6 +116,8 @@ def _load_native():
 
         from . import _torch_op
         globals().update({name: getattr(_torch_op, native) for name, native in _NATIVE.items()})
+        for name, native in _METHODS.items():
+            setattr(KvCache, name, _torch_op.method(globals()[native]))
     except ImportError as why:  # not built yet (or no torch): importing the package works, calling does not
         missing = str(why)
 
@@ -169,14 +173,13 @@ class KvCache:
             _load_native()
         _kv_append(self._h.value or 0, layer, k_new, v_new, pos, pos0, stream)  # noqa: F821
 
-    def append_rope(self, layer, q, k_new, v_new, **kw):
-        """b200_kv_append_rope: norm (where a weight is given) and rotation of q (n_streams, heads, n_new, hd; or None) and
-        k_new (n_streams, n_kv, n_new, hd), and k_new and v_new into the cache.  All float32 or all float16 CUDA tensors.
-        Keywords as in :func:`qk_norm_rope` (q_norm, k_norm, eps, rope_dims, rope_base, rope_scale, neox, pos, pos0, n_rows, out,
-        stream); the position of a row is its place in the cache.  Returns the rotated q, float16 unless `out` says otherwise."""
-        if "_kv_append_rope" not in globals():
-            _load_native()
-        return _kv_append_rope(self._h.value or 0, layer, q, k_new, v_new, **kw)  # noqa: F821
+    def append_rope(self, *args, **kw):
+        """b200_kv_append_rope: append_rope(layer, q, k_new, v_new, *, q_norm=None, k_norm=None, eps=1e-6, rope_dims=head_dim,
+        rope_base=10000.0, rope_scale=1.0, neox=True, pos=None, pos0=0, n_rows=None, out=None, stream=None).  Norm (where a weight is
+        given) and rotation of q (n_streams, heads, n_new, hd; or None) and k_new (n_streams, n_kv, n_new, hd), and k_new and v_new into the
+        cache; the position of a row is its place there.  Returns the rotated q, float16 unless `out` says otherwise."""
+        _load_native()
+        return _kv_append_rope(self, *args, **kw)  # noqa: F821
 
     def tensors(self, layer, n_rows):
         """Rows [0, n_rows) of a layer as torch tensors on the cache's memory: (K, V), each (n_streams, n_kv, n_rows, hd) float16 or
@@ -186,16 +189,12 @@ class KvCache:
             _load_native()
         return _kv_tensors(self._h.value or 0, self, layer, n_rows)  # noqa: F821
 
-    def read(self, layer, n_rows, pos=None, pos0=0, dtype=None, out=None, stream=None):
-        """b200_kv_read: rows pos[s] .. pos[s] + n_rows - 1 of every stream (`pos` an int32 CUDA tensor, else `pos0` for all) as values:
-        (K, V), each (n_streams, n_kv, n_rows, hd) float16, or float32 if `dtype` says so, or the pair `out`.  Rows outside
-        the cache are zeros."""
-        if "_kv_read" not in globals():
-            _load_native()
-        import torch
-        if dtype not in (None, torch.float16, torch.float32):
-            raise ValueError("dtype is torch.float16 or torch.float32")
-        return _kv_read(self._h.value or 0, layer, n_rows, pos, pos0, dtype is torch.float32, out, stream)  # noqa: F821
+    def read(self, *args, **kw):
+        """b200_kv_read: read(layer, n_rows, pos=None, pos0=0, dtype=None, out=None, stream=None).  Rows pos[s] .. pos[s] + n_rows - 1 of
+        every stream (`pos` an int32 CUDA tensor, else `pos0` for all) as values: (K, V), each (n_streams, n_kv, n_rows, hd) float16, or
+        float32 if `dtype` says so, or the pair `out`.  Rows outside the cache are zeros."""
+        _load_native()
+        return _kv_read(self, *args, **kw)  # noqa: F821
 
     def copy_stream(self, dst_stream, src_stream, n_rows, stream=None):
         """Fork a hypothesis: rows [0, n_rows) of every layer/head from one stream to another (kv_snapshot_pool)."""

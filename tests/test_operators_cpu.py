@@ -137,3 +137,28 @@ def test_python_refusals(b200):
         b200.qk_norm_rope()
     with pytest.raises(TypeError):
         b200.qk_norm_rope(x.numpy())
+
+
+class _NoCache:
+    """What the native methods see of a KvCache: its handle, here one that has been closed."""
+    _h = C.c_void_p()
+
+
+def test_cache_methods_refuse(b200):
+    from crispasr_b200 import op
+    op._load_native()
+    x = torch.zeros((1, 2, 3, 64))
+    assert op.KvCache.read.__doc__ and op.KvCache.append_rope.__doc__
+    with pytest.raises(b200.B200Error):
+        op.KvCache.read(_NoCache(), 0, 3)
+    for bad in (dict(), dict(layer=0), dict(layer=0, n_rows=1, rows=2), dict(layer=0, n_rows=1, dtype="f32"), dict(layer=0, n_rows=1, dtype=torch.int8)):
+        with pytest.raises((TypeError, ValueError)):
+            op.KvCache.read(_NoCache(), **bad)
+    with pytest.raises(TypeError, match="multiple values"):
+        op.KvCache.read(_NoCache(), 0, 3, layer=1)
+    with pytest.raises(ValueError, match="CUDA"):
+        op.KvCache.append_rope(_NoCache(), 0, None, x, x)
+    with pytest.raises(TypeError):
+        op.KvCache.append_rope(_NoCache(), 0, x, x)
+    with pytest.raises(TypeError, match="unexpected"):
+        op.KvCache.append_rope(_NoCache(), 0, None, x, x, base=3.0)
