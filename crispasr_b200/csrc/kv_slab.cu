@@ -80,8 +80,9 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
             }
         }
         // The rows of the next turn into L2 meanwhile: 16 x 407 rows of 8 heads into F16 15.5 -> 14.5 us, 8 x 1500 27.1 -> 26.0.  (Into Q8_0, whose
-        // arithmetic covers the loads, 1 %, and the attention behind 8 x 407 rows then starts 0.3 us later.)
-        if (U > 1 && TYPE == B200_TYPE_F16) {
+        // arithmetic covers the loads, 1 %, and the attention behind 8 x 407 rows then starts 0.3 us later.  Into Q4_0, with the smaller CTAs of
+        // launch_append, 15.2 -> 14.1, 24.7 -> 23.8 and, 1 x 2000 rows, 6.5 -> 5.2.)
+        if (U > 1 && TYPE != B200_TYPE_Q8_0) {
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int row = row0 + (U + u) * step + sub;
@@ -100,11 +101,13 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendArgs a) {
 template <int TYPE, bool V16>
 cudaError_t launch_append(AppendArgs a, int n_heads_total, cudaStream_t st) {
     // One token per stream: a warp per (stream, head).  Many rows: eight warps per CTA, four rows (of 128) in flight per warp, and
-    // no more CTAs than are resident at once (six per SM), so that a warp's next rows are requested without a new CTA's start.
+    // no more CTAs than are resident at once (six per SM), so that a warp's next rows are requested without a new CTA's start.  Into
+    // Q4_0, whose registers leave room for four, twice as many: three turns of shorter CTAs fill the SMs more evenly than one and a half.
+    constexpr int kPerSm = TYPE == B200_TYPE_Q4_0 ? 12 : 6;
     const int rpw = 32 / (a.hd / 8), n_new = a.n_new[0] > a.n_new[1] ? a.n_new[0] : a.n_new[1];
     const int units = (n_new + rpw - 1) / rpw;   // warp instructions per (stream, head)
     const int u = units >= 16 ? 2 : 1, warps = (units + u - 1) / u, per_block = warps < 8 ? warps : 8;
-    const int full = (warps + per_block - 1) / per_block, resident = (148 * 6 + 2 * n_heads_total - 1) / (2 * n_heads_total);
+    const int full = (warps + per_block - 1) / per_block, resident = (148 * kPerSm + 2 * n_heads_total - 1) / (2 * n_heads_total);
     a.chunks = full < resident ? full : resident;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.chunks * n_heads_total, 2);
