@@ -14,7 +14,7 @@
 //     product as two F16 terms, hi = f16(P d) and lo = f16(P d - hi), d the block's scale, formed and split by fused multiply-adds.
 //     With at most four query rows (FEW) the two terms are columns 0..3 and 4..7 of ONE MMA, whose other half would be padding;
 //     with more, two.  P is held up to 2^14 for that (its top is 2^10 at the running maximum plus the 2^4 by which the maximum may
-//     lag), so that lo keeps its bits above F16's smallest value; a warp that meets a scale of 2 or more lowers the top to 2^-4, for
+//     lag), so that lo keeps its bits above F16's smallest value; a warp that meets a scale of 2^e, e > 0, lowers the top to 2^(10 - e), for
 //     good, so that P d stays finite for every scale.  (Values whose scale is below 2^-17 lose some of the extra bits.)  The products of 32
 //     keys are summed by themselves and then added: the tensor cores cut a sum off at its last bit, which over thousands of keys showed as
 //     a shrinkage of 1e-6.
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
     constexpr int NBLK = HD / 32, RB = NBLK * 18, NS = kDecQ4Stages, WK = kDecQ4Keys, NT = WK / 16;
     constexpr int KT = WK * NW;                        // keys per tile
     constexpr int RAW = WK * RB + kDecQ4Skew;          // a warp's raw K or V bytes of a stage
-    constexpr float kTop = 10.0f, kLowTop = -4.0f, kGrow = 4.0f;   // log2: P at the running maximum, with scales of 2 and more, and how far the maximum may lag
+    constexpr float kTop = 10.0f, kGrow = 4.0f;   // log2: P at the running maximum while every scale is below 2, and how far the maximum may lag
     extern __shared__ __align__(128) uint8_t smem_raw[];
     __half* sQ = reinterpret_cast<__half*>(smem_raw);   // [8][HD], in the order the quads read them
     uint8_t* sRaw = smem_raw + 8 * HD * sizeof(__half);  // [NW][NS][K | V]
@@ -159,7 +159,6 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
     for (int blk = 0; blk < NBLK; blk++)
 #pragma unroll
         for (int mt = 0; mt < 2; mt++) o[blk][mt][0] = o[blk][mt][1] = o[blk][mt][2] = o[blk][mt][3] = 0.0f;
-    uint32_t large = 0x40004000u;   // the scale bits to look for while the top is kTop
     const uint32_t sel3 = t == 3 ? 0x5432u : 0x7654u;
     const uint32_t second = FEW && g >= 4 ? 0xFFFFFFFFu : 0u;   // FEW: columns 4..7 are the second terms
     auto rescale = [&](int j, float alpha) {
@@ -248,19 +247,27 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
 #pragma unroll
             for (int blk = 0; blk < NBLK; blk++) any_scale |= dv[nt][blk][0] | dv[nt][blk][1];
 
-        // ---- lazy running maximum, and the top of P: bit 14 of a half says 2 and more ----
+        // ---- lazy running maximum, and the top of P: bit 14 of a half says that a scale is 2 or more ----
         float lm[2] = {st[0][0], st[0][1]};
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int e = nt ? 0 : 2; e < 4; e++) lm[e & 1] = fmaxf(lm[e & 1], st[nt][e]);
-        if (__any_sync(0xffffffffu, lm[0] > bound[0] || lm[1] > bound[1] || (any_scale & large))) {
-            if (__any_sync(0xffffffffu, any_scale & large)) {
-                large = 0;
+        if (__any_sync(0xffffffffu, lm[0] > bound[0] || lm[1] > bound[1] || (any_scale & 0x40004000u))) {
+            if (__any_sync(0xffffffffu, any_scale & 0x40004000u)) {   // the largest exponent field E says d < 2^(E - 14)
+                uint32_t largest = 0;
 #pragma unroll
-                for (int j = 0; j < 2; j++) m_run[j] += top - kLowTop, rescale(j, 0x1p-14f);
-                static_assert(kTop - kLowTop == 14.0f, "");
-                top = kLowTop;
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int blk = 0; blk < NBLK; blk++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) largest = max(largest, max(dv[nt][blk][i] & 0x7C00u, (dv[nt][blk][i] >> 16) & 0x7C00u));
+                const float lower = fminf(top, 25.0f - (float)(__reduce_max_sync(0xffffffffu, largest) >> 10));
+                if (lower < top) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) m_run[j] += top - lower, rescale(j, exp2f(lower - top));
+                    top = lower;
+                }
             }
 #pragma unroll
             for (int j = 0; j < 2; j++) {

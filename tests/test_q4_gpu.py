@@ -513,3 +513,22 @@ def test_two_streams_and_two_graphs_at_once(b200):
     for i in range(2):
         assert torch.equal(held[i], outs[i])
     assert b200.lib().b200_device_status() == 0
+
+
+@pytest.mark.parametrize("size", [2.5, 40.0, 5000.0])
+@pytest.mark.parametrize("gqa,Tq", [(4, 1), (4, 3)])
+def test_serving_form_with_large_values(b200, size, gqa, Tq):
+    """Block scales of 2 and more: the range of the weights goes down by as much as they need, and not by more."""
+    rng = np.random.default_rng(int(size) + Tq)
+    kx, vx = (rng.standard_normal((1, 2, 4212, 128)).astype(np.float32) for _ in "kv")
+    vx *= size * rng.choice([0.05, 1.0], (1, 2, 4212, 1)).astype(np.float32)
+    k, v = quantize_q4_0(kx), quantize_q4_0(vx)
+    kf, vf = dequantize_q4_0(k), dequantize_q4_0(v)
+    q = randn_f16(rng, (1, 2 * gqa, Tq, 128))
+    for splits in (1, 0):
+        assert b200.lib().b200_set_decode_splits(splits) == 0
+        try:
+            got = gpu_op(b200, q, k, v, scale=0.1, kv_type=abi.Q4_0)
+        finally:
+            b200.lib().b200_set_decode_splits(0)
+        _exact(got, attention_f64(q, kf, vf, 0.1), f"{splits} splits")
