@@ -21,8 +21,8 @@
 //
 // What bounds it: instructions.  Per 16 keys of head_dim 128 a warp issues 385: 128 masks and multiply-adds of the nibbles, 52 from
 // and to shared memory (18-byte blocks come in words and halves), 28 for the scales of V, 24 that split P d, 20 MMAs; masks, shifts, byte
-// selections and half-precision arithmetic take two clocks each.  256 streams x 8 KV heads of up to 4096 keys (0.81 GB) 184 us, 4.4 TB/s or
-// 0.68 of the measured copy rate (all of them 4096 keys long: 262 us, 4.6 TB/s); in a loop of seconds, at the power limit, 205.  Stages
+// selections and half-precision arithmetic take two clocks each.  256 streams x 8 KV heads of up to 4096 keys (0.81 GB) 183 us, 4.5 TB/s or
+// 0.69 of the measured copy rate (all of them 4096 keys long: 262 us, 4.6 TB/s); in a loop of seconds, at the power limit, 205.  Stages
 // of 16 keys, whose waits, votes and addresses are per 16 keys, 238 us; 96 registers for a fifth CTA per SM, which leave no two m-tiles to
 // overlap, 218 where 128 registers took 198.
 constexpr int kDecQ4Stages = 2;
