@@ -290,7 +290,7 @@ void fill_turns(const b200_rope_params& r, uint64_t (&out)[kMaxHalf]) {
         for (int i = 0; i < r.n_dims / 2; i++) {
             long double f = (long double)r.freq_scale / two_pi * powl((long double)r.freq_base, -2.0L * i / r.n_dims);
             f -= floorl(f);
-            t.turns[i] = (uint64_t)(f * 18446744073709551616.0L);   // f < 1; a value that rounds up to 2^64 cannot arise: f has 64 bits
+            t.turns[i] = f < 1.0L ? (uint64_t)(f * 18446744073709551616.0L) : 0;   // (a tiny negative turn plus one rounds to a whole one)
         }
         t.n = r.n_dims, t.base = r.freq_base, t.scale = r.freq_scale;
     }

@@ -63,6 +63,15 @@ def test_far_positions(b200, p):
     assert_rows(got.cpu().numpy(), norm_rope_f64(y, None, pos, n_dims=128), False, f"position {p}")
 
 
+@pytest.mark.parametrize("scale", [-1.0, -0.25, -1e-30, 1e-30])
+def test_negative_and_tiny_frequencies(b200, scale):
+    """A negative turn is one less than a whole one; one too small to differ from it is none."""
+    rng = np.random.default_rng(5)
+    x = _rows(rng, (1, 2, 5, 64), torch.float32)
+    got, _ = b200.qk_norm_rope(x, pos0=321, rope_scale=scale)
+    assert_rows(got.cpu().numpy(), norm_rope_f64(x.cpu().numpy(), None, [321], n_dims=64, scale=scale), False, f"scale {scale}")
+
+
 def test_norm_of_small_and_zero_rows(b200):
     x = torch.zeros((1, 1, 4, 64), device="cuda")
     x[0, 0, 1], x[0, 0, 2, 5], x[0, 0, 3] = 1e-4, 1e-3, 1e18
