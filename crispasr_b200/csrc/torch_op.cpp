@@ -553,6 +553,18 @@ PyObject* qk_norm_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObject*
     END_HANDLE_TH_ERRORS
 }
 
+// A layer's index; one that passes 32 bits is no other layer's.
+bool layer_of(PyObject* o, int32_t* out) {
+    const long i = PyLong_AsLong(o);
+    if (i == -1 && PyErr_Occurred()) return false;
+    if (i != (int32_t)i) {
+        PyErr_SetString(PyExc_OverflowError, "layer is a 32-bit number");
+        return false;
+    }
+    *out = (int32_t)i;
+    return true;
+}
+
 // The address in a KvCache object (its `_h`, a ctypes pointer; null after close()).
 bool cache_of(PyObject* self, b200_kv_cache** out) {
     PyObject* h = PyObject_GetAttr(self, g_handle);
@@ -580,8 +592,8 @@ PyObject* kv_append_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObjec
     }
     b200_kv_cache* kv = nullptr;
     if (!cache_of(a[0], &kv)) return nullptr;
-    const long layer = PyLong_AsLong(a[1]);
-    if (PyErr_Occurred()) return nullptr;
+    int32_t layer = 0;
+    if (!layer_of(a[1], &layer)) return nullptr;
     RopeCall call;
     const at::Tensor *q = nullptr, *k = nullptr, *v = nullptr;
     if (!call.parse(names, a + n, "append_rope") || !rows_of(a[3], "k_new", nullptr, &k) || !rows_of(a[4], "v_new", k, &v)) return nullptr;
@@ -599,7 +611,7 @@ PyObject* kv_append_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObjec
     if (q && (!describe(*q, -1, &tq) || !(out = call.output(rOut, *q, at::kHalf, &made)) || !describe(*out, -1, &to))) return nullptr;
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = b200_kv_append_rope(kv, (int)layer, q ? &tq : nullptr, &tk, &tv, call.norm_p[0], call.norm_p[1], &call.params, call.pos, call.pos0, call.n_rows,
+    rc = b200_kv_append_rope(kv, layer, q ? &tq : nullptr, &tk, &tv, call.norm_p[0], call.norm_p[1], &call.params, call.pos, call.pos0, call.n_rows,
                              q ? &to : nullptr, call.stream);
     Py_END_ALLOW_THREADS
     if (rc) return raise_code(rc, "b200_kv_append_rope");
@@ -618,10 +630,11 @@ PyObject* kv_tensors_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     HANDLE_TH_ERRORS
     const b200_kv_cache* kv = (const b200_kv_cache*)PyLong_AsVoidPtr(a[0]);
-    const long layer = PyLong_AsLong(a[2]), rows = PyLong_AsLong(a[3]);
-    if (PyErr_Occurred()) return nullptr;
+    int32_t layer = 0;
+    const long rows = PyLong_AsLong(a[3]);
+    if (PyErr_Occurred() || !layer_of(a[2], &layer)) return nullptr;
     b200_tensor t[2];
-    const int rc = b200_kv_view(kv, (int)layer, rows, &t[0], &t[1]);
+    const int rc = b200_kv_view(kv, layer, rows, &t[0], &t[1]);
     if (rc) return raise_code(rc, "b200_kv_view");
     PyObject* views[2];
     for (int i = 0; i < 2; i++) {

@@ -162,3 +162,8 @@ def test_cache_methods_refuse(b200):
         op.KvCache.append_rope(_NoCache(), 0, x, x)
     with pytest.raises(TypeError, match="unexpected"):
         op.KvCache.append_rope(_NoCache(), 0, None, x, x, base=3.0)
+    for layer in (1 << 32, -(1 << 32)):   # not layer 0
+        with pytest.raises(OverflowError):
+            op.KvCache.append_rope(_NoCache(), layer, None, x, x)
+        with pytest.raises(OverflowError):
+            op._kv_tensors(0, _NoCache(), layer, 1)
