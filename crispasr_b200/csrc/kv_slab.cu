@@ -226,8 +226,18 @@ B200_API int b200_kv_create(const b200_kv_config* cfg, b200_kv_cache** out) {
         return B200_E_CUDA;
     }
     kv->base = (uint8_t*)(((uintptr_t)kv->arena + 1023) / 1024 * 1024);
-    // a cleared cache reads as zeros (whisper clears kv_pad at init, src/crispasr.cpp:1506)
-    if (cudaMemset(kv->arena, 0, total) != cudaSuccess) {
+    // A cleared cache reads as zeros (whisper clears kv_pad at init, src/crispasr.cpp:1506).  A memset of device memory is
+    // asynchronous to the host, and a non-blocking stream is ordered behind no other: the arena is handed out when it has been cleared, so that
+    // whatever stream writes its first rows, nothing overwrites them.  The stream is its own, which waits for no other's work.
+    cudaStream_t st = nullptr;
+    bool cleared = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess;
+    if (cleared) {
+        cleared = cudaMemsetAsync(kv->arena, 0, total, st) == cudaSuccess;
+        cleared = cudaStreamSynchronize(st) == cudaSuccess && cleared;
+        cudaStreamDestroy(st);
+    }
+    if (!cleared) {
+        cudaGetLastError();
         cudaFree(kv->arena);
         delete kv;
         return B200_E_CUDA;
