@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
     };
 
     for (int stage = 0, parity = 0; key0 < key_end; key0 += KT) {
-        if (!__any_sync(0xffffffffu, mbar_try_wait(bar + 8 * stage, (uint32_t)parity)) && !mbar_wait_bounded(bar + 8 * stage, (uint32_t)parity)) break;
+        // (every lane has to have seen the phase complete itself: that is what orders the copied bytes before its reads, a vote orders none)
+        if (!__all_sync(0xffffffffu, mbar_try_wait(bar + 8 * stage, (uint32_t)parity)) && !mbar_wait_bounded(bar + 8 * stage, (uint32_t)parity)) break;
         const uint8_t* rawK = stages + stage * 2 * RAW + kskew;
         const uint8_t* rawV = stages + stage * 2 * RAW + RAW + vskew;
 
