@@ -14,15 +14,19 @@
 //     product as two F16 terms, hi = f16(P d) and lo = f16(P d - hi), d the block's scale, formed and split by fused multiply-adds.
 //     With at most four query rows (FEW) the two terms are columns 0..3 and 4..7 of ONE MMA, whose other half would be padding;
 //     with more, two.  P is held up to 2^14 for that (its top is 2^10 at the running maximum plus the 2^4 by which the maximum may
-//     lag), so that lo keeps its bits above F16's smallest value; a warp that meets a scale of 2^e, e > 0, lowers the top to 2^(10 - e), for
-//     good, so that P d stays finite for every scale.  (Values whose scale is below 2^-17 lose some of the extra bits.)  The products of 32
+//     lag), so that lo keeps its bits above F16's smallest value.  The scales have to fit that range: a warp that meets one of 2^e, e > 0, lowers the
+//     top to 2^(10 - e), for good, so that P d stays finite; and where some run of 32 values of head_dim has only small scales (none of 2^-7 in the
+//     warp's first keys, or what a lowered top leaves small), these are multiplied by a power of two that its accumulators keep until the end (V of 1e-6: relative
+//     error 2e-7, without it 2e-4 to 7e-4).  Of a product of weight and scale what counts is kept to 2^-28 of the largest scale so far in its run of
+//     32.  256 streams x 4096 keys 182.1 -> 185.4 us by it, 64 ragged streams of six rows 29.6 -> 30.6, 97 keys 3.2 -> 3.4; a second copy of the key loop for such
+//     values, or scales rewritten in shared memory, cost 2 to 6 %.  The products of 32
 //     keys are summed by themselves and then added: the tensor cores cut a sum off at its last bit, which over thousands of keys showed as
 //     a shrinkage of 1e-6.
 //
 // What bounds it: instructions.  Per 16 keys of head_dim 128 a warp issues 385: 128 masks and multiply-adds of the nibbles, 52 from
 // and to shared memory (18-byte blocks come in words and halves), 28 for the scales of V, 24 that split P d, 20 MMAs; masks, shifts, byte
-// selections and half-precision arithmetic take two clocks each.  256 streams x 8 KV heads of up to 4096 keys (0.81 GB) 183 us, 4.5 TB/s or
-// 0.69 of the measured copy rate (all of them 4096 keys long: 262 us, 4.6 TB/s); in a loop of seconds, at the power limit, 205.  Stages
+// selections and half-precision arithmetic take two clocks each.  256 streams x 8 KV heads of up to 4096 keys (0.81 GB) 185 us, 4.4 TB/s or
+// 0.68 of the measured copy rate; in a loop of seconds, at the power limit, 205.  Stages
 // of 16 keys, whose waits, votes and addresses are per 16 keys, 238 us; 96 registers for a fifth CTA per SM, which leave no two m-tiles to
 // overlap, 218 where 128 registers took 198.
 constexpr int kDecQ4Stages = 2;
@@ -152,6 +156,14 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
     for (int j = 0; j < 2; j++) last[j] = a.causal ? min(len_b - 1, n_past + (FEW ? (2 * t + j) & 3 : row0 + 2 * t + j) / a.gqa) : len_b - 1;
 
     float top = kTop;
+    // Exponent fields of the largest scales so far, a byte per block of 32 values of head_dim; 15 (a scale of 1 to 2) stands for everything from 2^-7 on as
+    // long as nothing else was met.  What is missing to the top of P d's range is made up for by scales that enter the second product times 2^raised.
+    constexpr uint32_t kUnseen = 0x80808080u, kUsual = 0x0F0F0F0Fu;
+    uint32_t fields = kUnseen;
+    auto raised = [&](int blk) {   // (nothing has been summed while no scale was seen)
+        const int room = 25 - (int)top - (int)(fields >> (8 * blk) & 31u);
+        return fields != kUnseen && room > 3 ? room : 0;
+    };
     float m_run[2] = {ninf, ninf}, l_run[2] = {0.0f, 0.0f};   // reference (running maximum - top) and sum of rows 2t, 2t+1; the same on the lanes that share t
     float minus_m[2] = {0.0f, 0.0f}, bound[2] = {ninf, ninf};  // what is added to a score (nothing while the reference is -inf), and the largest that needs no new one
     float o[NBLK][2][4];   // [block][m-tile]: c0 / c1 = dim 32blk + 2g + mt of columns 2t / 2t+1, c2 / c3 = dim + 16, all times 2^-9
@@ -255,21 +267,6 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
 #pragma unroll
             for (int e = nt ? 0 : 2; e < 4; e++) lm[e & 1] = fmaxf(lm[e & 1], st[nt][e]);
         if (__any_sync(0xffffffffu, lm[0] > bound[0] || lm[1] > bound[1] || (any_scale & 0x40004000u))) {
-            if (__any_sync(0xffffffffu, any_scale & 0x40004000u)) {   // the largest exponent field E says d < 2^(E - 14)
-                uint32_t largest = 0;
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int blk = 0; blk < NBLK; blk++)
-#pragma unroll
-                        for (int i = 0; i < 2; i++) largest = max(largest, max(dv[nt][blk][i] & 0x7C00u, (dv[nt][blk][i] >> 16) & 0x7C00u));
-                const float lower = fminf(top, 25.0f - (float)(__reduce_max_sync(0xffffffffu, largest) >> 10));
-                if (lower < top) {
-#pragma unroll
-                    for (int j = 0; j < 2; j++) m_run[j] += top - lower, rescale(j, exp2f(lower - top));
-                    top = lower;
-                }
-            }
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 float rm = lm[j];
@@ -281,6 +278,72 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
                     m_run[j] = rm - top;
                 }
                 minus_m[j] = m_run[j] == ninf ? 0.0f : -m_run[j], bound[j] = m_run[j] + (top + kGrow);
+            }
+            bool fit = __any_sync(0xffffffffu, any_scale & 0x40004000u);
+            if (fields != kUsual) {
+                if (fields == kUnseen) {   // the warp's first keys
+                    uint32_t usual = 0;
+#pragma unroll
+                    for (int blk = 0; blk < NBLK; blk++) {
+                        uint32_t seen = 0;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) seen |= dv[nt][blk][0] | dv[nt][blk][1];
+                        usual |= seen & 0x60006000u ? 1u << blk : 0u;
+                    }
+                    if (__reduce_or_sync(0xffffffffu, usual) == (1u << NBLK) - 1) fields = kUsual;
+                    else fit = true;
+                } else {
+#pragma unroll
+                    for (int blk = 0; blk < NBLK; blk++) fit |= raised(blk) > 0;
+                }
+            }
+            if (fit) {   // exponent fields E of the largest scales: d < 2^(E - 14)
+                int was[NBLK], field[NBLK], most = 0;
+#pragma unroll
+                for (int blk = 0; blk < NBLK; blk++) {
+                    uint32_t largest = 0;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) largest = max(largest, max(dv[nt][blk][i] & 0x7C00u, (dv[nt][blk][i] >> 16) & 0x7C00u));
+                    was[blk] = raised(blk);
+                    field[blk] = max((int)(__reduce_max_sync(0xffffffffu, largest) >> 10), (int)(fields >> (8 * blk) & 31u));
+                    most = max(most, min(field[blk], 30));   // (an infinite scale has no range)
+                }
+                const float lower = fminf(top, 25.0f - (float)most);
+                if (lower < top) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        m_run[j] += top - lower, rescale(j, exp2f(lower - top));
+                        minus_m[j] = m_run[j] == ninf ? 0.0f : -m_run[j], bound[j] = m_run[j] + (lower + kGrow);
+                    }
+                    top = lower;
+                }
+                fields = 0;
+#pragma unroll
+                for (int blk = 0; blk < NBLK; blk++) {
+                    fields |= (uint32_t)field[blk] << (8 * blk);
+                    const int up = raised(blk);
+                    if (up != was[blk]) {
+                        const float f = exp2f((float)(up - was[blk]));
+#pragma unroll
+                        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[blk][mt][e] *= f;
+                    }
+                    if (up) {   // by two powers of two, of which F16 holds either
+                        bound[0] = bound[1] = ninf;   // (the next keys' scales come here too)
+                        const uint32_t a = (uint32_t)(15 + up / 2) << 10, b = (uint32_t)(15 + up - up / 2) << 10;
+                        const uint32_t a2 = a | a << 16, b2 = b | b << 16;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                const __half2 x = __hmul2(__hmul2(*reinterpret_cast<const __half2*>(&dv[nt][blk][i]), *reinterpret_cast<const __half2*>(&a2)), *reinterpret_cast<const __half2*>(&b2));
+                                dv[nt][blk][i] = *reinterpret_cast<const uint32_t*>(&x);
+                            }
+                    }
+                }
             }
         }
         // P^T as the B operand: (key g, columns 2t, 2t+1) -> (keys 2t, 2t+1, column g), the F16 values and what they leave of P
@@ -357,6 +420,9 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
         v += __shfl_xor_sync(0xffffffffu, v, 16);
         lq[j] = v;
     }
+    float unit[NBLK];
+#pragma unroll
+    for (int blk = 0; blk < NBLK; blk++) unit[blk] = __int_as_float((127 + 9 - raised(blk)) << 23);   // 2^(9 - raised)
     if (g == 0) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {   // (scores that are no numbers raise no maximum: the row must not pass for one without keys)
@@ -371,8 +437,8 @@ __global__ void __launch_bounds__(32 * NW, 16 / NW) fattn_decode_q4_kernel(const
         float* row = slab + (warp * 8 + 2 * t + j) * SLAB_STRIDE + 2 * g;
 #pragma unroll
         for (int blk = 0; blk < NBLK; blk++) {
-            *reinterpret_cast<float2*>(row + 32 * blk) = make_float2(o[blk][0][j] * 512.0f, o[blk][1][j] * 512.0f);
-            *reinterpret_cast<float2*>(row + 32 * blk + 16) = make_float2(o[blk][0][2 + j] * 512.0f, o[blk][1][2 + j] * 512.0f);
+            *reinterpret_cast<float2*>(row + 32 * blk) = make_float2(o[blk][0][j] * unit[blk], o[blk][1][j] * unit[blk]);
+            *reinterpret_cast<float2*>(row + 32 * blk + 16) = make_float2(o[blk][0][2 + j] * unit[blk], o[blk][1][2 + j] * unit[blk]);
         }
     }
     __syncthreads();

@@ -34,8 +34,9 @@
  *
  * Accuracy: operands of the tensor cores are F16, the weights P among them (relative 2^-11 each).  Decode over a Q4_0 cache
  * (head_dim 64 / 128, Tq * (H / Hkv) <= 16, no mask, softcap or index list, rows that follow one another from a 4-byte boundary on)
- * keeps P and the products to fp32: relative L2 below 2^-17.  Its rows at or beyond kv_len may hold anything; a key that only the
- * causal bound hides from a row has to be finite.
+ * keeps P and the products to fp32: relative L2 below 2^-17 in every run of 32 values of head_dim, whatever the size of V (what a key adds to a
+ * result is kept to 2^-28 of the largest block scale of V in that run: keys with scales far below those of keys that a row gives no weight
+ * lose bits).  Its rows at or beyond kv_len may hold anything; a key that only the causal bound hides from a row has to be finite.
  */
 #ifndef B200_FATTN_H
 #define B200_FATTN_H
