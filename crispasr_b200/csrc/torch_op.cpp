@@ -241,6 +241,16 @@ struct Operands {
     }
 };
 
+// While it lives, tensors made here come from the pool of the stream that a launch goes to: a block of the current stream's pool may still be in
+// use by that stream's earlier work, and would be handed out again while the launch is in flight.
+struct PoolOf {
+    c10::cuda::OptionalCUDAStreamGuard on_stream;
+    PoolOf(void* stream, c10::Device device) {
+        const cudaStream_t st = stream == (void*)cudaStreamLegacy ? nullptr : (cudaStream_t)stream;
+        if (st != c10::cuda::getCurrentCUDAStream(device.index()).stream()) on_stream.reset_stream(c10::cuda::getStreamFromExternal(st, device.index()));
+    }
+};
+
 struct Scratch {
     at::Tensor buf;
     c10::Device device;
@@ -253,12 +263,7 @@ void* scratch_alloc(void* user, size_t bytes) {
     Scratch* s = (Scratch*)user;
     if (s->given && s->given_bytes >= bytes) return s->given;
     try {
-        // The block comes from the pool of the stream that uses it: one of the current stream's pool may still be in use by
-        // that stream's earlier work, and would be handed out again while this launch is in flight.
-        c10::cuda::OptionalCUDAStreamGuard on_stream;
-        const cudaStream_t st = s->stream == (void*)cudaStreamLegacy ? nullptr : (cudaStream_t)s->stream;
-        if (st != c10::cuda::getCurrentCUDAStream(s->device.index()).stream())
-            on_stream.reset_stream(c10::cuda::getStreamFromExternal(st, s->device.index()));
+        const PoolOf pool(s->stream, s->device);
         s->buf = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, s->device, std::nullopt);
     } catch (...) {
         s->error = std::current_exception();
@@ -501,11 +506,12 @@ struct RopeCall {
         else if (!stream_of(v[rStream], &stream)) return false;
         return true;
     }
-    // The rows that a call writes: given, or made here.
+    // The rows that a call writes: given, or made here (after fill: the stream is known).
     const at::Tensor* output(RopeKey k, const at::Tensor& like, at::ScalarType type, at::Tensor* made) const {
         const at::Tensor* out = made;
-        if (!v[k]) *made = at::detail::empty_cuda(like.sizes(), type, like.device(), std::nullopt);
-        else if (!rows_of(v[k], kRopeNames[k], &like, &out)) return nullptr;
+        if (v[k]) return rows_of(v[k], kRopeNames[k], &like, &out) ? out : nullptr;
+        const PoolOf pool(stream, like.device());
+        *made = at::detail::empty_cuda(like.sizes(), type, like.device(), std::nullopt);
         return out;
     }
 };
@@ -516,7 +522,8 @@ const char kQkRopeDoc[] =
     "Norm of every head (where a weight is given) and rotation by position of q (streams, heads, rows, head_dim) and k (streams,\n"
     "kv heads, rows, head_dim), F32 or F16: (rotated q, rotated k or None), of q's type unless `out` and `k_out` say otherwise (they may\n"
     "be q and k).  Row i of stream s is at position pos[s] + i (`pos` an int32 CUDA tensor, else `pos0` for all); rows at or\n"
-    "beyond n_rows[s] (an int32 CUDA tensor) are zeros.  Asynchronous on `stream` (default: torch's current stream).";
+    "beyond n_rows[s] (an int32 CUDA tensor) are zeros.  Asynchronous on `stream` (default: torch's current stream), from whose pool the results are: a caller that\n"
+    "uses them on another stream orders the two and says so to the allocator (record_stream).";
 
 PyObject* qk_norm_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObject* names) {
     HANDLE_TH_ERRORS
@@ -581,7 +588,8 @@ const char kAppendRopeDoc[] =
     "            neox=True, pos=None, pos0=0, n_rows=None, out=None, stream=None)\n--\n\n"
     "Norm (where a weight is given) and rotation of q (n_streams, heads, n_new, hd; or None) and k_new (n_streams, n_kv, n_new, hd), and\n"
     "k_new and v_new into the cache.  All float32 or all float16 CUDA tensors.  Row i of stream s is at position pos[s] + i, which is\n"
-    "also its place in the cache; the other arguments as in qk_norm_rope.  Returns the rotated q, float16 unless `out` says otherwise.";
+    "also its place in the cache; the other arguments, and the order of streams, as in qk_norm_rope.  Returns the\n"
+    "rotated q, float16 unless `out` says otherwise.";
 
 // A method of KvCache: called with the object in front.
 PyObject* kv_append_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObject* names) {
@@ -663,7 +671,8 @@ PyObject* kv_tensors_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
 const char kReadDoc[] =
     "read(self, layer, n_rows, pos=None, pos0=0, dtype=None, out=None, stream=None)\n--\n\n"
     "Rows pos[s] .. pos[s] + n_rows - 1 of every stream (`pos` an int32 CUDA tensor, else `pos0` for all) as values: (K, V), each\n"
-    "(n_streams, n_kv, n_rows, hd) float16, or float32 if `dtype` says so, or the pair `out`.  Rows outside the cache are zeros.";
+    "(n_streams, n_kv, n_rows, hd) float16, or float32 if `dtype` says so, or the pair `out`.  Rows outside the cache are\n"
+    "zeros.  Asynchronous on `stream` (default: torch's current stream), from whose pool the results are.";
 
 // A method of KvCache: called with the object in front.
 PyObject* kv_read_py(PyObject*, PyObject* const* in, Py_ssize_t n, PyObject* names) {
@@ -714,8 +723,12 @@ PyObject* kv_read_py(PyObject*, PyObject* const* in, Py_ssize_t n, PyObject* nam
     const c10::Device device(at::kCUDA, (c10::DeviceIndex)device_of_cache(view[0].data));
     const c10::cuda::CUDAGuard guard(device);
     const int64_t sizes[4] = {view[0].ne[3], view[0].ne[2], rows, view[0].ne[0]};
+    void* st = nullptr;
+    if (!a[kOn]) st = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+    else if (!stream_of(a[kOn], &st)) return nullptr;
     at::Tensor out[2];
     if (!a[kOutPair]) {
+        const PoolOf pool(st, device);
         for (at::Tensor& o : out) o = at::detail::empty_cuda(sizes, type, device, std::nullopt);
     } else {
         if (!PyTuple_Check(a[kOutPair]) || PyTuple_GET_SIZE(a[kOutPair]) != 2) {
@@ -735,9 +748,6 @@ PyObject* kv_read_py(PyObject*, PyObject* const* in, Py_ssize_t n, PyObject* nam
     if (!describe(out[0], -1, &t[0]) || !describe(out[1], -1, &t[1])) return nullptr;
     const int32_t* pos = nullptr;
     if (a[kPos] && !table_of(a[kPos], "pos", out[0], sizes[0], &pos)) return nullptr;
-    void* st = nullptr;
-    if (!a[kOn]) st = c10::cuda::getCurrentCUDAStream(device.index()).stream();
-    else if (!stream_of(a[kOn], &st)) return nullptr;
     Py_BEGIN_ALLOW_THREADS
     rc = b200_kv_read(kv, (int)layer, &t[0], &t[1], pos, (int32_t)pos0, st);
     Py_END_ALLOW_THREADS

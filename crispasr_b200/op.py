@@ -177,7 +177,8 @@ class KvCache:
         """b200_kv_append_rope: append_rope(layer, q, k_new, v_new, *, q_norm=None, k_norm=None, eps=1e-6, rope_dims=head_dim,
         rope_base=10000.0, rope_scale=1.0, neox=True, pos=None, pos0=0, n_rows=None, out=None, stream=None).  Norm (where a weight is
         given) and rotation of q (n_streams, heads, n_new, hd; or None) and k_new (n_streams, n_kv, n_new, hd), and k_new and v_new into the
-        cache; the position of a row is its place there.  Returns the rotated q, float16 unless `out` says otherwise."""
+        cache; the position of a row is its place there.  Returns the rotated q, float16 unless `out` says otherwise, from the pool
+        of the stream that the call goes to: a caller that uses it on another stream orders the two and says so to the allocator (record_stream)."""
         _load_native()
         return _kv_append_rope(self, *args, **kw)  # noqa: F821
 
@@ -192,7 +193,8 @@ class KvCache:
     def read(self, *args, **kw):
         """b200_kv_read: read(layer, n_rows, pos=None, pos0=0, dtype=None, out=None, stream=None).  Rows pos[s] .. pos[s] + n_rows - 1 of
         every stream (`pos` an int32 CUDA tensor, else `pos0` for all) as values: (K, V), each (n_streams, n_kv, n_rows, hd) float16, or
-        float32 if `dtype` says so, or the pair `out`.  Rows outside the cache are zeros."""
+        float32 if `dtype` says so, or the pair `out`; results are from the pool of the stream that the call goes to.  Rows outside the cache
+        are zeros."""
         _load_native()
         return _kv_read(self, *args, **kw)  # noqa: F821
 

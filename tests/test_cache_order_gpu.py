@@ -38,3 +38,33 @@ def test_first_rows_of_a_new_cache_on_a_non_blocking_stream(b200, type_, how):
         kv.close()
         torch.cuda.synchronize()
     small.close()
+
+
+def _calls(b200, side):
+    """Each call that makes its results, on `side`: (results, all of one shape and type)."""
+    S, H, n, hd = 2, 5, 8191, 128
+    q = torch.randn((S, H, n, hd), device="cuda", dtype=torch.float16)
+    kv = b200.KvCache(abi.Q8_0, hd, H, n_layers=1, max_ctx=n, n_streams=S)
+    return {"qk_norm_rope": lambda: b200.qk_norm_rope(q, q, stream=side), "append_rope": lambda: (kv.append_rope(0, q, q, q, stream=side),),
+            "read": lambda: kv.read(0, n, stream=side)}, q
+
+
+@pytest.mark.parametrize("call", ["qk_norm_rope", "append_rope", "read"])
+@pytest.mark.parametrize("handle", ["stream", "integer", "current"])
+def test_results_come_from_the_pool_of_the_launch_stream(b200, call, handle):
+    """A block that the current stream has given back, and may still be working on, is not handed to a launch on another stream."""
+    side = torch.cuda.Stream()
+    calls, like = _calls(b200, None if handle == "current" else side if handle == "stream" else side.cuda_stream)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    back = [torch.empty_like(like) for _ in range(2)]
+    freed = {x.data_ptr() for x in back}
+    del back
+    results = calls[call]()
+    at = {x.data_ptr() for x in results}
+    assert (at <= freed) if handle == "current" else not at & freed
+    torch.cuda.synchronize()
+    del results
+    with torch.cuda.stream(side):   # ... and goes back to that pool
+        again = {torch.empty_like(like).data_ptr() for _ in range(1)}
+    assert handle == "current" or again <= at
