@@ -358,6 +358,18 @@ PyObject* forward_host_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObject*
     END_HANDLE_TH_ERRORS
 }
 
+// A layer's index or a row's; one that passes 32 bits is no other's.
+bool index_of(PyObject* o, const char* what, int32_t* out) {
+    const long i = PyLong_AsLong(o);
+    if (i == -1 && PyErr_Occurred()) return false;
+    if (i != (int32_t)i) {
+        PyErr_Format(PyExc_OverflowError, "%s is a 32-bit number", what);
+        return false;
+    }
+    *out = (int32_t)i;
+    return true;
+}
+
 // (cache address, layer, k_new, v_new, pos, pos0, stream)
 PyObject* kv_append_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 7) {
@@ -366,13 +378,13 @@ PyObject* kv_append_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     HANDLE_TH_ERRORS
     b200_kv_cache* kv = (b200_kv_cache*)PyLong_AsVoidPtr(a[0]);
-    const long layer = PyLong_AsLong(a[1]);
-    if (PyErr_Occurred()) return nullptr;
+    int32_t layer = 0, pos0 = 0;
+    if (PyErr_Occurred() || !index_of(a[1], "layer", &layer)) return nullptr;
     PyObject* p0 = PyNumber_Long(a[5]);   // int(pos0): floats as well
     if (!p0) return nullptr;
-    const long pos0 = PyLong_AsLong(p0);
+    const bool ok = index_of(p0, "pos0", &pos0);
     Py_DECREF(p0);
-    if (PyErr_Occurred()) return nullptr;
+    if (!ok) return nullptr;
     const at::Tensor *k = tensor_of(a[2], "k_new"), *v = k ? tensor_of(a[3], "v_new") : nullptr;
     b200_tensor tk, tv;
     if (!v || !describe(*k, -1, &tk) || !describe(*v, -1, &tv)) return nullptr;
@@ -391,7 +403,7 @@ PyObject* kv_append_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
     else if (!stream_of(a[6], &st)) return nullptr;
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = b200_kv_append(kv, (int)layer, &tk, &tv, pos, (int32_t)pos0, st);
+    rc = b200_kv_append(kv, layer, &tk, &tv, pos, pos0, st);
     Py_END_ALLOW_THREADS
     if (rc) return raise_code(rc, "b200_kv_append");
     Py_RETURN_NONE;
@@ -560,18 +572,6 @@ PyObject* qk_norm_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObject*
     END_HANDLE_TH_ERRORS
 }
 
-// A layer's index; one that passes 32 bits is no other layer's.
-bool layer_of(PyObject* o, int32_t* out) {
-    const long i = PyLong_AsLong(o);
-    if (i == -1 && PyErr_Occurred()) return false;
-    if (i != (int32_t)i) {
-        PyErr_SetString(PyExc_OverflowError, "layer is a 32-bit number");
-        return false;
-    }
-    *out = (int32_t)i;
-    return true;
-}
-
 // The address in a KvCache object (its `_h`, a ctypes pointer; null after close()).
 bool cache_of(PyObject* self, b200_kv_cache** out) {
     PyObject* h = PyObject_GetAttr(self, g_handle);
@@ -601,7 +601,7 @@ PyObject* kv_append_rope_py(PyObject*, PyObject* const* a, Py_ssize_t n, PyObjec
     b200_kv_cache* kv = nullptr;
     if (!cache_of(a[0], &kv)) return nullptr;
     int32_t layer = 0;
-    if (!layer_of(a[1], &layer)) return nullptr;
+    if (!index_of(a[1], "layer", &layer)) return nullptr;
     RopeCall call;
     const at::Tensor *q = nullptr, *k = nullptr, *v = nullptr;
     if (!call.parse(names, a + n, "append_rope") || !rows_of(a[3], "k_new", nullptr, &k) || !rows_of(a[4], "v_new", k, &v)) return nullptr;
@@ -640,7 +640,7 @@ PyObject* kv_tensors_py(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const b200_kv_cache* kv = (const b200_kv_cache*)PyLong_AsVoidPtr(a[0]);
     int32_t layer = 0;
     const long rows = PyLong_AsLong(a[3]);
-    if (PyErr_Occurred() || !layer_of(a[2], &layer)) return nullptr;
+    if (PyErr_Occurred() || !index_of(a[2], "layer", &layer)) return nullptr;
     b200_tensor t[2];
     const int rc = b200_kv_view(kv, layer, rows, &t[0], &t[1]);
     if (rc) return raise_code(rc, "b200_kv_view");
