@@ -25,7 +25,7 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
 }
 // Four Q4_0 nibbles in the low halves of a word's bytes: trunc(x * id + 8.5), at most 15, for x * id in [-8, 8] up to a rounding.
 // The sum is formed on top of 2^22 and rounded towards zero, which leaves a whole number of halves (bit 0 of the result) and cannot
-// reach an integer that the exact sum does not reach; 16 becomes 15.  (A block with values that are no numbers gets some nibble.)
+// reach an integer that the exact sum does not reach; 16 becomes 15.  (A NaN gets nibble 14.)
 __device__ __forceinline__ uint32_t nibbles_of(float x0, float x1, float x2, float x3, float id) {
     constexpr float kBase = 4194304.0f + 8.5f;
     const uint32_t w = low_bytes(__float_as_uint(__fmaf_rz(x0, id, kBase)), __float_as_uint(__fmaf_rz(x1, id, kBase)), __float_as_uint(__fmaf_rz(x2, id, kBase)),

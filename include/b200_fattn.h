@@ -338,7 +338,9 @@ B200_API int b200_kv_view(const b200_kv_cache* kv, int layer, int64_t n_rows, b2
  * F32 rows k_new/v_new [hd, n_new, n_kv_heads, n_streams] (device, generic strides) to the cache
  * type and stores them at rows pos[s] .. pos[s]+n_new-1 of each stream s (`pos` is a device
  * array [n_streams], or NULL meaning `pos0` for all).  A Q4_0 block's scale is its value of largest magnitude (the first
- * of them) / -8, its nibbles trunc(x / scale + 8.5), at most 15.  Asynchronous on `cuda_stream`.
+ * of them) / -8, its nibbles trunc(x / scale + 8.5), at most 15.  A NaN does not count for the scale of its block and becomes some number of the
+ * block's range (in Q8_0 a zero; a Q4_0 block of nothing else reads as NaN): a caller that has to see it looks ahead of the cache.  A Q4_0 block with an infinity,
+ * or whose scale passes F16's largest value, reads as infinities and NaN.  Asynchronous on `cuda_stream`.
  */
 B200_API int b200_kv_append(b200_kv_cache* kv, int layer, const b200_tensor* k_new, const b200_tensor* v_new,
                             const int32_t* pos, int32_t pos0, void* cuda_stream);
