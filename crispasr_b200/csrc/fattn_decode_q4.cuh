@@ -23,10 +23,11 @@
 //     keys are summed by themselves and then added: the tensor cores cut a sum off at its last bit, which over thousands of keys showed as
 //     a shrinkage of 1e-6.
 //
-// What bounds it: instructions.  Per 16 keys of head_dim 128 a warp issues 385: 128 masks and multiply-adds of the nibbles, 52 from
+// What bounds it: the issue of instructions by four warps per scheduler, whose own fixed latencies leave a third of the slots empty (78 % of them used on a full SM,
+// 67 % over the launch; no pipe is full: ALU 50 %, LSU 37, FMA 26, HMMA 22).  Per 16 keys of head_dim 128 a warp issues 388: 128 masks and multiply-adds of the nibbles, 52 from
 // and to shared memory (18-byte blocks come in words and halves), 28 for the scales of V, 24 that split P d, 20 MMAs; masks, shifts, byte
 // selections and half-precision arithmetic take two clocks each.  256 streams x 8 KV heads of up to 4096 keys (0.81 GB) 185 us, 4.4 TB/s or
-// 0.68 of the measured copy rate; in a loop of seconds, at the power limit, 205.  Stages
+// 0.68 of the measured copy rate; in a loop of seconds, at the power limit, 207.  Stages
 // of 16 keys, whose waits, votes and addresses are per 16 keys, 238 us; 96 registers for a fifth CTA per SM, which leave no two m-tiles to
 // overlap, 218 where 128 registers took 198.
 constexpr int kDecQ4Stages = 2;
